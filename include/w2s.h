@@ -406,6 +406,67 @@ int w2s_map_labels(const float* src, float* dst, long n, int num_classes, void* 
 int w2s_causal_normalize_host(const double* x, long n, double sampling_freq, double tau_seconds, double eps, double outlier_sigma,
                               double baseline_tau_seconds, double min_sigma, double* out, uint8_t* outlier);
 
+/* ---- operators of a causal state space mixer (short_conv.hip, ssm_scan.hip, add_norm.hip) ---------------------------------------------
+ * No call of the reference stands behind these: they are a recurrent alternative to its SequenceCNN (models/wav2sleep.py:349-390), with a
+ * form for one position at a time.  Activations are fp32, bf16 or fp16 (`dtype`), channels-last, channel stride 1, any other strides (given
+ * in ELEMENTS); outputs are contiguous; parameters and states of the scan are fp32.  lengths: device int32 [B] or NULL; position t of
+ * sequence b exists if t < lengths[b] (clamped to [0, L] on the device): outputs and gradients behind it are 0 and inputs there are not read. */
+#define W2S_F32 0
+#define W2S_BF16 1
+#define W2S_F16 2
+
+/* y[b,t,d] = act(bias[d] + sum_k w[d][k] x[b, t-(K-1)+k, d]), positions before 0 from state [B][K-1][D] (NULL: zeros); state_out (or NULL):
+ * the last K-1 inputs before the sequence's end, from `state` where the sequence is shorter.  1 <= K <= 8.  act: 0 none, 1 SiLU */
+typedef struct w2s_short_conv_args {
+  const void* x; const void* state; const float* w; const float* bias; const int32_t* lengths;
+  void* y; void* state_out;
+  const void* gy; const void* gstate;      /* backward: gradients of y and of state_out (either may be NULL) */
+  void* gx; void* gstate_in; float* gw; float* gbias; float* part;
+  int64_t sx_b, sx_l, sg_b, sg_l;          /* strides of x and gy */
+  int32_t B, L, D, K, dtype, act;
+} w2s_short_conv_args;
+int w2s_short_conv_fwd(const w2s_short_conv_args* a, void* stream);
+int64_t w2s_short_conv_part(const w2s_short_conv_args* a);   /* floats of `part` that w2s_short_conv_bwd needs */
+int w2s_short_conv_bwd(const w2s_short_conv_args* a, void* stream);   /* gx, gw, gbias / gstate_in (may be NULL) */
+/* one position: x [B][D] (row stride sx_b), state [B][K-1][D] -> y [B][D], state_out (may be `state` itself) */
+int w2s_short_conv_step(const w2s_short_conv_args* a, void* stream);
+
+/* Selective scan: delta = softplus(dt + dt_bias) (softplus = 0: no softplus), h_t = exp(delta_t A) h_{t-1} + delta_t u_t B_t,
+ * y_t = (sum_n C_t[n] h_t[n] + D u_t) silu(z_t).  u, dt, z, y [B][L][D]; Bm, Cm [B][L][G][N] (state index contiguous; channel d belongs to
+ * group d / (D/G)); A [D][N]; D, dt_bias [D]; h0, h_out [B][D][N].  D, dt_bias, z, h0, h_out, lengths may be NULL.  1 <= N <= 64. */
+typedef struct w2s_ssm_args {
+  const void* u; const void* dt; const void* z; const void* Bm; const void* Cm;
+  const float* A; const float* Dp; const float* dt_bias; const float* h0; const int32_t* lengths;
+  void* y; float* h_out;
+  float* ckpt;                             /* states that the forward leaves for the backward (NULL in inference), w2s_ssm_ckpt floats */
+  const void* gy; const float* gh;         /* backward: gradients of y and of h_out (either may be NULL) */
+  void* gu; void* gdt; void* gz; void* gB; void* gC; float* gA; float* gD; float* gbias; float* gh0;
+  void* ws;                                /* scratch, w2s_ssm_ws bytes */
+  int64_t su_b, su_l, sdt_b, sdt_l, sz_b, sz_l, sB_b, sB_l, sB_g, sC_b, sC_l, sC_g, sg_b, sg_l;
+  int32_t B, L, D, N, G, dtype, softplus, reserved;
+} w2s_ssm_args;
+int64_t w2s_ssm_ckpt(const w2s_ssm_args* a);
+int64_t w2s_ssm_ws(const w2s_ssm_args* a, int backward);
+int w2s_ssm_scan_fwd(const w2s_ssm_args* a, void* stream);
+int w2s_ssm_scan_bwd(const w2s_ssm_args* a, void* stream);   /* gu, gdt, gz (with z), gB, gC, gA; gD, gbias, gh0 may be NULL */
+/* one position: u, dt, z, y [B][D] (row strides s*_b), Bm, Cm [B][G][N]; h_out may be h0 itself */
+int w2s_ssm_step(const w2s_ssm_args* a, void* stream);
+
+/* r = x + res (fp32 sum), y = r / sqrt(mean(r^2) + eps) * w over rows of C.  x, y: dtype; res, r: rdtype (dtype or W2S_F32); res = r = NULL:
+ * y from x alone.  fp8 != 0: y is e4m3 (OCP), one byte an element, y[row][c] scale[row] ~ the normalised value, scale = max|.| / 448 (1 for
+ * a row of zeros).  rstd (or NULL): 1 / sqrt(mean + eps) per row, fp32, for the backward. */
+typedef struct w2s_add_norm_args {
+  const void* x; const void* res; const float* w; void* y; void* r; float* scale; float* rstd;
+  const void* gy; const void* gr; void* gx; void* gres; float* gw; float* part;   /* backward; gr, gres, gw may be NULL */
+  int64_t rows, ldx, ldres, ldgy, ldgr;    /* outputs are contiguous */
+  int32_t C, dtype, rdtype, fp8;
+  float eps; int32_t reserved;
+} w2s_add_norm_args;
+int w2s_add_norm_fwd(const w2s_add_norm_args* a, void* stream);
+int64_t w2s_add_norm_part(const w2s_add_norm_args* a);       /* floats of `part` that w2s_add_norm_bwd needs */
+/* the sum comes from x + res again; x = NULL: from res alone (r saved in fp32).  gx: dtype; gres: rdtype (NULL: not wanted or the same as gx) */
+int w2s_add_norm_bwd(const w2s_add_norm_args* a, void* stream);
+
 const char* w2s_version(void);
 /* Integer ABI number of this header: bumped whenever a signature or the meaning of an argument changes (round 5: 6; round 6: 7).  The host refuses a
  * library whose number differs from the one it was written against (wav2sleep_amd/lib.py), so a stale build_alt/ or W2S_LIB library is

@@ -1,0 +1,379 @@
+// Root-mean-square norm with the residual's addition: r = x + res, y = r rstd w, rstd = 1 / sqrt(mean(r^2) + eps), y in 16 / 32 bits or in e4m3
+// with one scale a row.  Three or four elements moved per element and five flops: bound by HBM, so a row is read once and lives in registers
+// (G lanes x NV vectors) between the sum of squares and the product; only rows beyond 256 lanes x 8 vectors, and widths or pointers that
+// no vector access fits, are read twice (the second time from L2) by the looped kernel.  The sum is fp32 and y comes from it before r is rounded.
+#include "mix_io.h"
+
+namespace {
+
+constexpr float kFp8Max = 448.0f;   // largest finite e4m3 value
+
+// sum / maximum over the G lanes of a row: inside a wave by lane exchanges, over a workgroup's four waves through LDS
+template <int G, bool MAX> __device__ __forceinline__ float row_reduce(float v, float* red) {
+  if constexpr (G <= 64) {
+    return MAX ? mix_group_max<G>(v) : mix_group_sum<G>(v);
+  } else {
+    v = MAX ? mix_group_max<64>(v) : mix_group_sum<64>(v);
+    constexpr int W = G / 64;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
+    return v;
+  }
+}
+
+template <int N> __device__ __forceinline__ void store_fp8(uint8_t* p, const float* v) {   // v within +-448 or NaN
+  if constexpr (N == 1) {
+    *p = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xff);
+  } else {
+    static_assert(N % 4 == 0, "four codes a word");
+    uint32_t w[N / 4];
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+      w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], q, true);
+    }
+    if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  }
+}
+
+// y / scale into [-448, 448]; a NaN stays one (fmin / fmax would drop it)
+__device__ __forceinline__ float to_fp8_range(float y, float scale) {
+  const float q = y / scale;
+  return q != q ? q : fminf(fmaxf(q, -kFp8Max), kFp8Max);
+}
+
+__device__ __forceinline__ float fp8_scale(float top) { return top > 0.0f ? top / kFp8Max : (top == top ? 1.0f : top); }
+
+template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ __launch_bounds__(256) void add_norm_fwd_kernel(w2s_add_norm_args a) {
+  __shared__ float red[4];
+  constexpr int RPB = 256 / G;
+  const int lane = threadIdx.x % G, C = a.C;
+  const int64_t row = (int64_t)blockIdx.x * RPB + threadIdx.x / G;
+  if (G <= 64 && row >= a.rows) return;
+  const T* x = (const T*)a.x + row * a.ldx;
+  const RT* res = a.res ? (const RT*)a.res + row * a.ldres : nullptr;
+  float v[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * G + lane) * VEC;
+    if (c < C) {
+      mix_load<T, VEC>(x + c, v[j]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
+    }
+  }
+  if (res) {
+    float q[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * VEC;
+      if (c < C) mix_load<RT, VEC>(res + c, q[j]);
+    }
+    RT* r = (RT*)a.r + row * C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * VEC;
+      if (c < C) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] += q[j][i];
+        mix_store<RT, VEC>(r + c, v[j]);
+      }
+    }
+  }
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) s = __builtin_fmaf(v[j][i], v[j][i], s);
+  const float rstd = 1.0f / __builtin_sqrtf(row_reduce<G, false>(s, red) / (float)C + a.eps);
+  if (a.rstd && lane == 0) a.rstd[row] = rstd;
+  float top = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * G + lane) * VEC;
+    if (c < C) {
+      float w[VEC];
+      mix_load<float, VEC>(a.w + c, w);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        v[j][i] *= rstd * w[i];
+        if (FP8) top = v[j][i] != v[j][i] || top != top ? __builtin_nanf("") : fmaxf(top, __builtin_fabsf(v[j][i]));
+      }
+      if (!FP8) mix_store<T, VEC>((T*)a.y + row * C + c, v[j]);
+    }
+  }
+  if (FP8) {
+    const float bad = top != top ? 1.0f : 0.0f;
+    top = row_reduce<G, true>(bad != 0.0f ? 0.0f : top, red);
+    if (row_reduce<G, true>(bad, red) != 0.0f) top = __builtin_nanf("");
+    const float scale = fp8_scale(top);
+    if (lane == 0) a.scale[row] = scale;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * VEC;
+      if (c < C) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[j][i] = to_fp8_range(v[j][i], scale);
+        store_fp8<VEC>((uint8_t*)a.y + row * C + c, v[j]);
+      }
+    }
+  }
+}
+
+// any width, any alignment: a workgroup per row, one element a lane, the row's sum formed again in every pass
+template <typename T, typename RT, bool FP8> __global__ __launch_bounds__(256) void add_norm_fwd_loop_kernel(w2s_add_norm_args a) {
+  __shared__ float red[4];
+  const int C = a.C;
+  const int64_t row = blockIdx.x;
+  const T* x = (const T*)a.x + row * a.ldx;
+  const RT* res = a.res ? (const RT*)a.res + row * a.ldres : nullptr;
+  auto sum_at = [&](int c) { return res ? (float)x[c] + (float)res[c] : (float)x[c]; };
+  float s = 0.0f;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    const float v = sum_at(c);
+    s = __builtin_fmaf(v, v, s);
+    if (res) ((RT*)a.r)[row * C + c] = (RT)v;
+  }
+  const float rstd = 1.0f / __builtin_sqrtf(row_reduce<256, false>(s, red) / (float)C + a.eps);
+  if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+  if (!FP8) {
+    for (int c = threadIdx.x; c < C; c += 256) ((T*)a.y)[row * C + c] = (T)(sum_at(c) * (rstd * a.w[c]));
+    return;
+  }
+  float top = 0.0f, bad = 0.0f;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    const float v = sum_at(c) * (rstd * a.w[c]);
+    if (v != v) bad = 1.0f;
+    else top = fmaxf(top, __builtin_fabsf(v));
+  }
+  top = row_reduce<256, true>(top, red);
+  if (row_reduce<256, true>(bad, red) != 0.0f) top = __builtin_nanf("");
+  const float scale = fp8_scale(top);
+  if (threadIdx.x == 0) a.scale[row] = scale;
+  for (int c = threadIdx.x; c < C; c += 256) {
+    const float q = to_fp8_range(sum_at(c) * (rstd * a.w[c]), scale);
+    store_fp8<1>((uint8_t*)a.y + row * C + c, &q);
+  }
+}
+
+// Backward, n = r rstd: gr_total = rstd (gy w - n mean(gy w n)) + gr goes to both addends; gw = sum over rows of gy n.  A workgroup takes rows
+// blockIdx, blockIdx + gridDim, ... and keeps its share of gw in registers; the shares are joined in a fixed order.
+template <typename T, typename RT, int VEC, int G, int NV> __global__ __launch_bounds__(256) void add_norm_bwd_kernel(w2s_add_norm_args a) {
+  __shared__ float red[4];
+  __shared__ float acc[G < 256 ? 256 * VEC : 1];
+  constexpr int RPB = 256 / G;
+  const int lane = threadIdx.x % G, C = a.C;
+  float gw[NV][VEC], w[NV][VEC];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int c = (j * G + lane) * VEC;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) gw[j][i] = w[j][i] = 0.0f;
+    if (c < C) mix_load<float, VEC>(a.w + c, w[j]);
+  }
+  for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
+    const int64_t row = r0 + threadIdx.x / G;
+    const bool on = row < a.rows;   // (a whole group of lanes; with G = 256 always)
+    float n[NV][VEC], g[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * VEC;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) n[j][i] = g[j][i] = 0.0f;
+      if (on && c < C) {
+        if (a.x) mix_load<T, VEC>((const T*)a.x + row * a.ldx + c, n[j]);
+        if (a.res) {
+          float q[VEC];
+          mix_load<RT, VEC>((const RT*)a.res + row * a.ldres + c, q);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) n[j][i] += q[i];
+        }
+        if (a.gy) mix_load<T, VEC>((const T*)a.gy + row * a.ldgy + c, g[j]);
+      }
+    }
+    const float rstd = on ? a.rstd[row] : 0.0f;
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        n[j][i] *= rstd;
+        gw[j][i] = __builtin_fmaf(g[j][i], n[j][i], gw[j][i]);
+        g[j][i] *= w[j][i];
+        s = __builtin_fmaf(g[j][i], n[j][i], s);
+      }
+    const float m = row_reduce<G, false>(s, red) / (float)C;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (j * G + lane) * VEC;
+      if (on && c < C) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] = 0.0f;
+        if (a.gr) mix_load<RT, VEC>((const RT*)a.gr + row * a.ldgr + c, o);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] += rstd * __builtin_fmaf(-n[j][i], m, g[j][i]);
+        if (a.gx) mix_store<T, VEC>((T*)a.gx + row * C + c, o);
+        if (a.gres) mix_store<RT, VEC>((RT*)a.gres + row * C + c, o);
+      }
+    }
+  }
+  if (!a.gw) return;
+  float* part = a.part + (int64_t)blockIdx.x * C;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if constexpr (G == 256) {
+      const int c = (j * G + lane) * VEC;
+      if (c < C) mix_store<float, VEC>(part + c, gw[j]);
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) acc[i * 256 + threadIdx.x] = gw[j][i];
+      __syncthreads();
+      for (int q = threadIdx.x; q < G * VEC; q += 256) {
+        const int l = q / VEC, i = q % VEC, c = (j * G + l) * VEC + i;
+        if (c < C) {
+          float t = 0.0f;
+          for (int p = 0; p < RPB; ++p) t += acc[i * 256 + p * G + l];
+          part[c] = t;
+        }
+      }
+    }
+  }
+}
+
+template <typename T, typename RT> __global__ __launch_bounds__(256) void add_norm_bwd_loop_kernel(w2s_add_norm_args a) {
+  __shared__ float red[4];
+  const int C = a.C;
+  float* part = a.gw ? a.part + (int64_t)blockIdx.x * C : nullptr;
+  if (part)
+    for (int c = threadIdx.x; c < C; c += 256) part[c] = 0.0f;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = a.x ? (const T*)a.x + row * a.ldx : nullptr;
+    const RT* res = a.res ? (const RT*)a.res + row * a.ldres : nullptr;
+    const T* gy = a.gy ? (const T*)a.gy + row * a.ldgy : nullptr;
+    const RT* gr = a.gr ? (const RT*)a.gr + row * a.ldgr : nullptr;
+    const float rstd = a.rstd[row];
+    auto n_at = [&](int c) { return ((x ? (float)x[c] : 0.0f) + (res ? (float)res[c] : 0.0f)) * rstd; };
+    auto g_at = [&](int c) { return gy ? (float)gy[c] : 0.0f; };
+    float s = 0.0f;
+    for (int c = threadIdx.x; c < C; c += 256) s = __builtin_fmaf(g_at(c) * a.w[c], n_at(c), s);
+    const float m = row_reduce<256, false>(s, red) / (float)C;
+    for (int c = threadIdx.x; c < C; c += 256) {   // (a column of `part` belongs to one thread)
+      const float n = n_at(c), g = g_at(c);
+      if (part) part[c] = __builtin_fmaf(g, n, part[c]);
+      const float o = (gr ? (float)gr[c] : 0.0f) + rstd * __builtin_fmaf(-n, m, g * a.w[c]);
+      if (a.gx) ((T*)a.gx)[row * C + c] = (T)o;
+      if (a.gres) ((RT*)a.gres)[row * C + c] = (RT)o;
+    }
+  }
+}
+
+__global__ __launch_bounds__(1024) void add_norm_reduce_kernel(const float* part, int nparts, int C, float* gw) {
+  __shared__ float red[16][64];
+  const int col = blockIdx.x * 64 + (threadIdx.x & 63), row = threadIdx.x >> 6;
+  float v = 0.0f;
+  if (col < C)
+    for (int p = row; p < nparts; p += 16) v += part[(int64_t)p * C + col];
+  red[row][threadIdx.x & 63] = v;
+  __syncthreads();
+  if (row == 0 && col < C) {
+    for (int q = 1; q < 16; ++q) v += red[q][threadIdx.x];
+    gw[col] = v;
+  }
+}
+
+int esize(int dtype) { return dtype == W2S_F32 ? 4 : 2; }
+
+bool valid(const w2s_add_norm_args* a) {
+  return a && a->w && a->rows >= 0 && a->rows <= 0x7fffffff && a->C >= 1 && a->dtype >= 0 && a->dtype <= 2 &&
+         (a->rdtype == a->dtype || a->rdtype == W2S_F32);
+}
+
+// elements a lane's access: 16 bytes of T where widths, rows and pointers allow, else 1
+int vector_of(const w2s_add_norm_args* a) {
+  const int v = 16 / esize(a->dtype);
+  if (a->C % v || a->ldx % v || a->ldres % v || a->ldgy % v || a->ldgr % v) return 1;
+  const void* ps[] = {a->x, a->res, a->w, a->r, a->gy, a->gr, a->gx, a->gres};
+  for (const void* p : ps)
+    if ((uintptr_t)p % 16) return 1;
+  if ((uintptr_t)a->y % (a->fp8 ? 8 : 16)) return 1;
+  return v;
+}
+
+// workgroups of the backward: enough for 8 waves a SIMD quad on every CU, at most one per row group
+int bwd_blocks(const w2s_add_norm_args* a) {
+  const int64_t n = a->rows < 1 ? 1 : a->rows;
+  return (int)(n < 1024 ? n : 1024);
+}
+
+template <typename T, typename RT, int VEC, int G, int NV> int go(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
+  const int64_t groups = (a->rows + 256 / G - 1) / (256 / G);
+  if (bwd) {
+    const int nb = bwd_blocks(a);
+    add_norm_bwd_kernel<T, RT, VEC, G, NV><<<nb, 256, 0, st>>>(*a);
+  } else if (a->fp8) {
+    add_norm_fwd_kernel<T, RT, true, VEC, G, NV><<<(unsigned)groups, 256, 0, st>>>(*a);
+  } else {
+    add_norm_fwd_kernel<T, RT, false, VEC, G, NV><<<(unsigned)groups, 256, 0, st>>>(*a);
+  }
+  return W2S_OK;
+}
+
+template <typename T, typename RT> int by_width(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int units = vector_of(a) == V ? a->C / V : 1 << 30;   // lanes' accesses a row
+  if (units <= 16) return go<T, RT, V, 16, 1>(a, bwd, st);
+  if (units <= 32) return go<T, RT, V, 32, 1>(a, bwd, st);
+  if (units <= 64) return go<T, RT, V, 64, 1>(a, bwd, st);
+  if (units <= 128) return go<T, RT, V, 64, 2>(a, bwd, st);
+  if (units <= 256) return go<T, RT, V, 256, 1>(a, bwd, st);
+  if (units <= 512) return go<T, RT, V, 256, 2>(a, bwd, st);
+  if (units <= 1024) return go<T, RT, V, 256, 4>(a, bwd, st);
+  if (bwd) {
+    add_norm_bwd_loop_kernel<T, RT><<<bwd_blocks(a), 256, 0, st>>>(*a);
+  } else if (a->fp8) {
+    add_norm_fwd_loop_kernel<T, RT, true><<<(unsigned)a->rows, 256, 0, st>>>(*a);
+  } else {
+    add_norm_fwd_loop_kernel<T, RT, false><<<(unsigned)a->rows, 256, 0, st>>>(*a);
+  }
+  return W2S_OK;
+}
+
+int dispatch(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
+  const bool wide_r = a->rdtype != a->dtype;
+  switch (a->dtype) {
+    case W2S_F32: by_width<float, float>(a, bwd, st); break;
+    case W2S_BF16: wide_r ? by_width<bf16_t, float>(a, bwd, st) : by_width<bf16_t, bf16_t>(a, bwd, st); break;
+    case W2S_F16: wide_r ? by_width<half_t, float>(a, bwd, st) : by_width<half_t, half_t>(a, bwd, st); break;
+  }
+  if (bwd && a->gw) add_norm_reduce_kernel<<<(a->C + 63) / 64, 1024, 0, st>>>(a->part, bwd_blocks(a), a->C, a->gw);
+  W2S_CHECK_LAUNCH();
+  return W2S_OK;
+}
+
+}  // namespace
+
+extern "C" int w2s_add_norm_fwd(const w2s_add_norm_args* a, void* stream) {
+  if (!valid(a)) return W2S_EINVAL;
+  if (a->rows == 0) return W2S_OK;
+  if (!a->x || !a->y || (!a->res) != (!a->r) || (a->fp8 && !a->scale)) return W2S_EINVAL;
+  return dispatch(a, false, (hipStream_t)stream);
+}
+
+extern "C" int64_t w2s_add_norm_part(const w2s_add_norm_args* a) {
+  if (!valid(a)) return W2S_EINVAL;
+  return (int64_t)bwd_blocks(a) * a->C;
+}
+
+extern "C" int w2s_add_norm_bwd(const w2s_add_norm_args* a, void* stream) {
+  if (!valid(a) || a->fp8 || (a->gw && !a->part)) return W2S_EINVAL;
+  if (a->rows > 0 && ((!a->x && !a->res) || !a->rstd)) return W2S_EINVAL;
+  return dispatch(a, true, (hipStream_t)stream);   // no rows: the sums are still written (zeros)
+}

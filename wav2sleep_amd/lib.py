@@ -55,11 +55,31 @@ class WgradArgs(C.Structure):
                                     'pro_g', 'pro_h', 'nslab', 'split_precision')]
 
 
+class ShortConvArgs(C.Structure):
+    _fields_ = [(n, _fp) for n in ('x', 'state', 'w', 'bias', 'lengths', 'y', 'state_out', 'gy', 'gstate', 'gx', 'gstate_in', 'gw', 'gbias', 'part')] + \
+               [(n, C.c_int64) for n in ('sx_b', 'sx_l', 'sg_b', 'sg_l')] + [(n, _i32) for n in ('B', 'L', 'D', 'K', 'dtype', 'act')]
+
+
+class SsmArgs(C.Structure):
+    _fields_ = [(n, _fp) for n in ('u', 'dt', 'z', 'Bm', 'Cm', 'A', 'Dp', 'dt_bias', 'h0', 'lengths', 'y', 'h_out', 'ckpt', 'gy', 'gh', 'gu', 'gdt', 'gz',
+                                   'gB', 'gC', 'gA', 'gD', 'gbias', 'gh0', 'ws')] + \
+               [(n, C.c_int64) for n in ('su_b', 'su_l', 'sdt_b', 'sdt_l', 'sz_b', 'sz_l', 'sB_b', 'sB_l', 'sB_g', 'sC_b', 'sC_l', 'sC_g', 'sg_b', 'sg_l')] + \
+               [(n, _i32) for n in ('B', 'L', 'D', 'N', 'G', 'dtype', 'softplus', 'reserved')]
+
+
+class AddNormArgs(C.Structure):
+    _fields_ = [(n, _fp) for n in ('x', 'res', 'w', 'y', 'r', 'scale', 'rstd', 'gy', 'gr', 'gx', 'gres', 'gw', 'part')] + \
+               [(n, C.c_int64) for n in ('rows', 'ldx', 'ldres', 'ldgy', 'ldgr')] + [(n, _i32) for n in ('C', 'dtype', 'rdtype', 'fp8')] + \
+               [('eps', C.c_float), ('reserved', _i32)]
+
+
 EXPORTS = ['w2s_conv_tile', 'w2s_conv_cfg', 'w2s_linear_pf_takes', 'w2s_seq_conv', 'w2s_conv_forward', 'w2s_wgrad', 'w2s_wgrad_max_blocks', 'w2s_wgrad_slabs_per_block_of', 'w2s_wgrad_grid_y', 'w2s_wgrad_slabs_per_block', 'w2s_wgrad_reduce', 'w2s_wgrad_reduce_batch', 'w2s_repack', 'w2s_repack_batch', 'w2s_repack_bf16',
            'w2s_conv_fwd_fused', 'w2s_conv_fwd_fused_tile', 'w2s_bwd_fused', 'w2s_bwd_wide', 'w2s_bwd_wide_tile', 'w2s_bwd_wide_groups', 'w2s_bwd_fused_h', 'w2s_gp_stats_h', 'w2s_enc_first_bwd_h', 'w2s_bwd_fused_w1', 'w2s_bwd_fused_wd', 'w2s_enc_first_wgrad', 'w2s_enc_first_dwd', 'w2s_enc_first_stats', 'w2s_bwd_fused_tile', 'w2s_bwd_fused_folds_residual', 'w2s_stats_finalize', 'w2s_enc_first_fwd', 'w2s_enc_first_join', 'w2s_enc_first_bwd', 'w2s_gp_stats',
            'w2s_layernorm_fwd', 'w2s_layernorm_bwd', 'w2s_bias_grad', 'w2s_colsum', 'w2s_colsum_batch', 'w2s_gelu_bwd_rows', 'w2s_fill_rows', 'w2s_add_rows', 'w2s_causal_normalize_host', 'w2s_eltwise',
            'w2s_attn_fwd', 'w2s_attn_bwd', 'w2s_head_fwd', 'w2s_ce_fwd_bwd', 'w2s_ce_count', 'w2s_ce_wave', 'w2s_ce_final', 'w2s_head_bwd', 'w2s_sumsq_partial',
-           'w2s_clip_coef', 'w2s_adamw', 'w2s_ema_update', 'w2s_swap', 'w2s_zscore', 'w2s_augment', 'w2s_map_labels', 'w2s_token_masks', 'w2s_cls_scatter', 'w2s_copy_rows', 'w2s_zero', 'w2s_affine_act', 'w2s_rownorm_fwd', 'w2s_attn_generic_fwd', 'w2s_norm_act_bwd_part', 'w2s_norm_act_bwd_apply', 'w2s_rownorm_bwd_blocks', 'w2s_rownorm_bwd', 'w2s_attn_generic_bwd', 'w2s_norm_fold', 'w2s_norm_bwd_coef', 'w2s_affine_act_join', 'w2s_affine_act_join_bwd', 'w2s_conv1_fwd', 'w2s_conv1_wgrad_parts', 'w2s_conv1_wgrad', 'w2s_version', 'w2s_abi_version']
+           'w2s_clip_coef', 'w2s_adamw', 'w2s_ema_update', 'w2s_swap', 'w2s_zscore', 'w2s_augment', 'w2s_map_labels', 'w2s_token_masks', 'w2s_cls_scatter', 'w2s_copy_rows', 'w2s_zero', 'w2s_affine_act', 'w2s_rownorm_fwd', 'w2s_attn_generic_fwd', 'w2s_norm_act_bwd_part', 'w2s_norm_act_bwd_apply', 'w2s_rownorm_bwd_blocks', 'w2s_rownorm_bwd', 'w2s_attn_generic_bwd', 'w2s_norm_fold', 'w2s_norm_bwd_coef', 'w2s_affine_act_join', 'w2s_affine_act_join_bwd', 'w2s_conv1_fwd', 'w2s_conv1_wgrad_parts', 'w2s_conv1_wgrad',
+           'w2s_short_conv_fwd', 'w2s_short_conv_part', 'w2s_short_conv_bwd', 'w2s_short_conv_step', 'w2s_ssm_ckpt', 'w2s_ssm_ws', 'w2s_ssm_scan_fwd', 'w2s_ssm_scan_bwd',
+           'w2s_ssm_step', 'w2s_add_norm_fwd', 'w2s_add_norm_part', 'w2s_add_norm_bwd', 'w2s_version', 'w2s_abi_version']
 
 ABI_VERSION = 8   # include/w2s.h W2S_ABI_VERSION
 _lib = None
@@ -103,6 +123,8 @@ def load():
                 raise RuntimeError(f'{LIB_PATH} does not export {name}')
         lib.w2s_version.restype = C.c_char_p
         lib.w2s_abi_version.restype = C.c_int
+        for name in ('w2s_short_conv_part', 'w2s_ssm_ckpt', 'w2s_ssm_ws', 'w2s_add_norm_part'):
+            getattr(lib, name).restype = C.c_int64
         if lib.w2s_abi_version() != ABI_VERSION:   # a stale W2S_LIB / build_alt library would be called with shifted arguments
             raise RuntimeError(f'{LIB_PATH} has ABI {lib.w2s_abi_version()}, this host was written against {ABI_VERSION} (include/w2s.h): rebuild it')
         _lib = lib
@@ -761,6 +783,32 @@ def rownorm_bwd_blocks(rows) -> int:
 def rownorm_bwd(g, ldg, x, ldx, gamma, beta, gx, ldgx, part, rows, Cc, eps, rms=False, act=0, slope=0.01):
     _chk(load().w2s_rownorm_bwd(_f(g), ldg, _f(x), ldx, _f(gamma), _f(beta), _f(gx), ldgx, _f(part), C.c_long(rows), Cc, C.c_float(eps), int(rms),
                                 act, C.c_float(slope), _stream()), 'w2s_rownorm_bwd')
+
+
+# ---- operators of a causal state space mixer (mixer_ops.py holds the public functions): `a` is a filled ShortConvArgs / SsmArgs / AddNormArgs,
+#      whose tensors `ptr` has turned into addresses
+IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # W2S_F32 / W2S_BF16 / W2S_F16
+
+
+def ptr(t):
+    """address of a device tensor for a descriptor field (None: NULL); remembers its device for the launch's check, as _p does"""
+    if t is None:
+        return None
+    if not t.is_cuda:
+        raise W2SError('wav2sleep_amd kernels need device tensors (no CPU path)')
+    _tls.dev = t.device.index
+    return t.data_ptr()
+
+
+def mixer_size(name: str, a, *more) -> int:
+    n = getattr(load(), name)(C.byref(a), *more)
+    if n < 0:
+        raise W2SError(f'{name} failed with code {n}')
+    return n
+
+
+def mixer_call(name: str, a):
+    _chk(getattr(load(), name)(C.byref(a), _stream()), name)
 
 
 def version() -> str:
