@@ -791,24 +791,32 @@ IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # W2S_F32 
 
 
 def ptr(t):
-    """address of a device tensor for a descriptor field (None: NULL); remembers its device for the launch's check, as _p does"""
-    if t is None:
-        return None
-    if not t.is_cuda:
-        raise W2SError('wav2sleep_amd kernels need device tensors (no CPU path)')
-    _tls.dev = t.device.index
-    return t.data_ptr()
+    """address of a tensor for a descriptor field (None: NULL); the caller has checked its device"""
+    return None if t is None else t.data_ptr()
+
+
+_entry = {}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, '_cuda_getCurrentRawStream') else (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _resolve(name):
+    f = getattr(load(), name)
+    _entry[name] = f
+    return f
 
 
 def mixer_size(name: str, a, *more) -> int:
-    n = getattr(load(), name)(C.byref(a), *more)
+    n = (_entry.get(name) or _resolve(name))(C.byref(a), *more)
     if n < 0:
         raise W2SError(f'{name} failed with code {n}')
     return n
 
 
-def mixer_call(name: str, a):
-    _chk(getattr(load(), name)(C.byref(a), _stream()), name)
+def mixer_call(name: str, a, dev: int):
+    """launch on the current stream of device `dev`, which is the current device (mixer_ops._On)"""
+    rc = (_entry.get(name) or _resolve(name))(C.byref(a), C.c_void_p(_raw_stream(dev)))
+    if rc != 0:
+        _chk(rc, name)
 
 
 def version() -> str:
