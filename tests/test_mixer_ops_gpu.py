@@ -625,6 +625,9 @@ def test_refusals():
                 f(*args)
     with pytest.raises(E):
         W.add_rms_norm_8bit(x.clone().requires_grad_(True), rnd(1, 8))
+    far = torch.zeros(5 * (1 << 22) + 64, device='cuda').as_strided((2, 6, 8), (8, 1 << 22, 1))   # positions further apart than the offsets inside a tile reach
+    with pytest.raises(E):
+        W.ssm_scan(**{**good, 'u': far})
     u = p['u'].clone().requires_grad_(True)   # first order only
     y = W.ssm_scan(**{**good, 'u': u})
     g, = torch.autograd.grad(y.sum(), u, create_graph=True)

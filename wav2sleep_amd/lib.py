@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 import subprocess
+import sys
 
 import torch
 
@@ -87,7 +88,7 @@ _lib = None
 
 def build(verbose: bool = False) -> str:
     """Compile libw2s_hip.so for gfx950 in-tree (hipcc cross-compiles without a GPU)."""
-    r = subprocess.run(['make', '-C', CSRC, '-j8'], capture_output=True, text=True)
+    r = subprocess.run(['make', '-C', CSRC, '-j8', f'PYTHON={sys.executable}'], capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError('building libw2s_hip.so failed:\n' + r.stdout[-4000:] + r.stderr[-4000:])
     if verbose:
@@ -785,38 +786,21 @@ def rownorm_bwd(g, ldg, x, ldx, gamma, beta, gx, ldgx, part, rows, Cc, eps, rms=
                                 act, C.c_float(slope), _stream()), 'w2s_rownorm_bwd')
 
 
-# ---- operators of a causal state space mixer (mixer_ops.py holds the public functions): `a` is a filled ShortConvArgs / SsmArgs / AddNormArgs,
-#      whose tensors `ptr` has turned into addresses
+# ---- operators of a causal state space mixer: mixer_ops.py holds the public functions, csrc/torch_ops.cpp their host side
 IO_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}   # W2S_F32 / W2S_BF16 / W2S_F16
+TORCH_OPS_PATH = os.path.join(_HERE, '_w2s_torch.so')
+_TORCH_OPS_ENTRIES = ['w2s_short_conv_fwd', 'w2s_short_conv_part', 'w2s_short_conv_bwd', 'w2s_short_conv_step', 'w2s_ssm_ckpt', 'w2s_ssm_ws', 'w2s_ssm_scan_fwd',
+                      'w2s_ssm_scan_bwd', 'w2s_ssm_step', 'w2s_add_norm_fwd', 'w2s_add_norm_part', 'w2s_add_norm_bwd']
 
 
-def ptr(t):
-    """address of a tensor for a descriptor field (None: NULL); the caller has checked its device"""
-    return None if t is None else t.data_ptr()
-
-
-_entry = {}
-_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, '_cuda_getCurrentRawStream') else (lambda i: torch.cuda.current_stream(i).cuda_stream)
-
-
-def _resolve(name):
-    f = getattr(load(), name)
-    _entry[name] = f
-    return f
-
-
-def mixer_size(name: str, a, *more) -> int:
-    n = (_entry.get(name) or _resolve(name))(C.byref(a), *more)
-    if n < 0:
-        raise W2SError(f'{name} failed with code {n}')
-    return n
-
-
-def mixer_call(name: str, a, dev: int):
-    """launch on the current stream of device `dev`, which is the current device (mixer_ops._On)"""
-    rc = (_entry.get(name) or _resolve(name))(C.byref(a), C.c_void_p(_raw_stream(dev)))
-    if rc != 0:
-        _chk(rc, name)
+def load_torch_ops():
+    """The extension module of csrc/torch_ops.cpp, bound to this library's kernels; raises loudly if it is not there."""
+    if not os.path.exists(TORCH_OPS_PATH):
+        raise RuntimeError(f'{TORCH_OPS_PATH} not found: run `python -c "import __graft_entry__ as g; g.build()"` (or `make -C wav2sleep_amd/csrc`)')
+    dll = load()
+    from . import _w2s_torch
+    _w2s_torch.bind([C.cast(getattr(dll, n), C.c_void_p).value for n in _TORCH_OPS_ENTRIES], W2SError)
+    return _w2s_torch
 
 
 def version() -> str:
