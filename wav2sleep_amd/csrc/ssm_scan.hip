@@ -18,7 +18,6 @@
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int kWaves = 8;
 
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -35,11 +34,9 @@ __device__ __forceinline__ float quad_bcast(float v, int k) {   // lane k of the
 // a loop would otherwise carry one 64-bit address a lane for every access.  Between the walks over a tile it keeps what a walk can cheaply form again (broadcasts, LDS reads,
 // states) from being carried to the next one in registers, of which the decays take a quarter
 __device__ __forceinline__ void forget(float& v) { asm("" : "+v"(v)); }
-template <int M, int N> __device__ __forceinline__ void forget(float (&v)[M][N]) {
+template <int N> __device__ __forceinline__ void forget(float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < M; ++i)
-#pragma unroll
-    for (int k = 0; k < N; ++k) forget(v[i][k]);
+  for (int i = 0; i < N; ++i) forget(v[i]);
 }
 __device__ __forceinline__ int forgotten(int v) {
   asm("" : "+v"(v));
@@ -68,14 +65,21 @@ __device__ __forceinline__ float sum_quads_of_row(float v) {   // over the four 
   return v;
 }
 
-// tile shapes by states per lane: TT positions a wave x CPL channels a quad x NPL states a lane
-template <int NPL> struct FwdShape { static constexpr int CPL = 1, TT = NPL <= 4 ? 16 : 64 / NPL; };                  // 64 decays a lane
-template <int NPL> struct BwdShape { static constexpr int CPL = NPL <= 2 ? 2 : 1, TT = NPL <= 8 ? 8 : 4; };
+// tile shapes by states per lane: W waves, TT positions a wave.  Sixteen waves of few positions hide each other's LDS and barrier waits (four a SIMD, which
+// 128 registers a lane allow); from eight states a lane on the registers of a walk leave two a SIMD.
+#ifndef FW
+#define FW 16
+#define FT 8
+#define BW 16
+#define BT 4
+#endif
+template <int NPL> struct FwdShape { static constexpr int W = NPL <= 4 ? FW : 8, TT = NPL <= 4 ? FT : 64 / NPL; };
+template <int NPL> struct BwdShape { static constexpr int W = NPL <= 4 ? BW : 8, TT = NPL <= 4 ? BT : NPL <= 8 ? 8 : 4; };
 
 struct Plan {
-  int dg, ncb, ntile, nseg, tps, nck, vbc, vch;   // channels a group, channel blocks a group, tiles, segments, tiles a segment, checkpoints a sequence; B/C by fours, channels by twos
-  float *segh, *segs;                             // [B][nseg][D][NP] end states, [B][nseg][D] sums of delta (nseg > 1)
-  float *part_bc, *part_a;                        // backward: [channel block][B][L][G][2 NP], [B nseg][D][N + 2]
+  int dg, ncb, ntile, nseg, tps, nck, vbc;   // channels a group, channel blocks a group, tiles, segments, tiles a segment, checkpoints a sequence; B / C: 0 one by one, 1 by fours, 2 and N needs no padding
+  float *segh, *segs;                        // [B][nseg][D][NP] end states, [B][nseg][D] sums of delta (nseg > 1)
+  float *part_bc, *part_a;                   // backward: [channel block][B][L][G][2 NP], [B nseg][D][N + 2]
 };
 
 // Workgroups go to the 8 XCDs in turn; neighbouring channel blocks share cache lines, so each XCD (its own L2) gets a run of consecutive ones.
@@ -97,275 +101,282 @@ __device__ __forceinline__ Where where_of(const w2s_ssm_args& a, const Plan& p) 
   return w;
 }
 
-// CPL adjacent channels of one position at a wave-uniform address + 32-bit lane offsets (scalar base, vector offset: no 64-bit arithmetic a lane).
-// VCH: the channels come in whole aligned pairs, one access and one offset; else one each, a channel that does not exist reading the group's last
-template <typename T, int CPL, bool VCH> __device__ __forceinline__ void load_ch(const T* base, const unsigned (&off)[CPL], float* v) {
-  if constexpr (VCH) {
-    mix_load<T, CPL>(base + (unsigned)forgotten(off[0]), v);
+// One channel's values of a tensor [L][channels], four positions to a quad (lane q has positions 4 i + q of its wave's TT): a wave-uniform running row, moved
+// on a tile at a time, and one 32-bit lane offset, so that an access is a scalar base and an offset and costs no 64-bit arithmetic a lane.
+template <typename T> struct Column {
+  T* row;           // position 0 of this wave's TT in the current tile, the group's first channel
+  int64_t four, tile;
+  unsigned off;
+  __device__ __forceinline__ void start(const void* base, int64_t sb, int64_t sl, int b, int channel0, int t, int tile_step, int q, int ch) {
+    row = (T*)base + b * sb + t * sl + channel0;
+    four = 4 * sl;
+    tile = tile_step * sl;
+    off = (unsigned)(q * sl) + ch;
+  }
+  __device__ __forceinline__ void move() { row += tile; }
+  __device__ __forceinline__ T get(int i) const { return (row + i * four)[(unsigned)forgotten(off)]; }
+  __device__ __forceinline__ void put(int i, float v) const { (row + i * four)[(unsigned)forgotten(off)] = (T)v; }
+};
+// (values stay in the memory's type until a tile is worked on: a conversion here would wait for the load that it is to hide)
+template <typename T, int NI> __device__ __forceinline__ void get_all(const Column<const T>& c, bool whole, int left, int q, T (&v)[NI]) {   // left: positions up to L
+  if (whole) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) v[i] = c.get(i);
   } else {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) v[c] = (float)base[(unsigned)forgotten(off[c])];
+    for (int i = 0; i < NI; ++i)
+      if (4 * i + q < left) v[i] = c.get(i);
   }
 }
-template <typename T, int CPL, bool VCH> __device__ __forceinline__ void store_ch(T* base, const unsigned (&off)[CPL], int n, const float* v) {   // n: how many exist
-  if constexpr (VCH) {
-    if (n > 0) mix_store<T, CPL>(base + (unsigned)forgotten(off[0]), v);
+template <typename T, int NI> __device__ __forceinline__ void put_all(const Column<T>& c, bool whole, int left, int q, bool on, const float (&v)[NI]) {
+  if (whole) {
+    if (on) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) c.put(i, v[i]);
+    }
   } else {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c)
-      if (c < n) base[(unsigned)forgotten(off[c])] = (T)v[c];
+    for (int i = 0; i < NI; ++i)
+      if (on && 4 * i + q < left) c.put(i, v[i]);
   }
-}
-template <int CPL> __device__ __forceinline__ void offsets(unsigned (&off)[CPL], int64_t stride, int q, int ch, int last) {
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) off[c] = (unsigned)(q * stride) + ch + (c < last ? c : last);
 }
 
-// B and C of a tile on their way from global memory to LDS: unit = four states of one position of one of the two
-template <typename T, int NP, int TILE> struct StageBC {
-  static constexpr int UNITS = TILE * NP / 4 * 2, PER = (UNITS + kWaves * 64 - 1) / (kWaves * 64);
-  float v[PER][4];
-  __device__ __forceinline__ void load(const w2s_ssm_args& a, const Plan& p, const T* Bg, const T* Cg, int t0, bool with_c) {   // Bg, Cg: the group's first state
-    const T* b0 = Bg + (int64_t)t0 * a.sB_l;
-    const T* c0 = Cg + (int64_t)t0 * a.sC_l;
+// B and C of a tile on their way from global memory to LDS: unit = four states of one position of one of the two; a wave's 64 units of a round lie in one
+template <typename T, int NP, int TILE, int W> struct StageBC {
+  static constexpr int HALF = TILE * NP / 4, PER = (2 * HALF + W * 64 - 1) / (W * 64);
+  static_assert(HALF % 64 == 0, "a wave's units are all of B or all of C");
+  const T *rowB, *rowC;   // the tile's first position
+  int64_t tileB, tileC;
+  unsigned off[PER];
+  typedef typename mix_vec<T, 4>::type V;
+  V v[PER];
+  __device__ __forceinline__ void start(const w2s_ssm_args& a, const Where& at, int t, int tile_step, int w, int lane) {
+    rowB = (const T*)a.Bm + at.b * a.sB_b + at.g * a.sB_g + t * a.sB_l;
+    rowC = (const T*)a.Cm + at.b * a.sC_b + at.g * a.sC_g + t * a.sC_l;
+    tileB = tile_step * a.sB_l;
+    tileC = tile_step * a.sC_l;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = k * kWaves * 64 + (int)threadIdx.x;
-      const int half = UNITS / 2, isc = i >= half, r = isc ? i - half : i, row = r / (NP / 4), n = r % (NP / 4) * 4;
+      const int u0 = (k * W + w) * 64, isc = u0 >= HALF, r = u0 - isc * HALF + lane;
+      off[k] = r / (NP / 4) * (unsigned)(isc ? a.sC_l : a.sB_l) + r % (NP / 4) * 4;
+    }
+  }
+  __device__ __forceinline__ void move() {
+    rowB += tileB;
+    rowC += tileC;
+  }
+  __device__ __forceinline__ void load(const w2s_ssm_args& a, int vbc, int left, bool with_c, int w, int lane) {   // left: positions of the tile up to L
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[k][e] = 0.0f;
-      if (i < UNITS && (with_c || !isc) && t0 + row < a.L && n < a.N) {
-        const T* src = isc ? c0 + (unsigned)forgotten(row * (int)a.sC_l + n) : b0 + (unsigned)forgotten(row * (int)a.sB_l + n);
-        if (p.vbc) {
-          mix_load<T, 4>(src, v[k]);
-        } else {
+    for (int k = 0; k < PER; ++k) {
+      const int u0 = (k * W + w) * 64, isc = u0 >= HALF;
+      if (u0 >= 2 * HALF || (isc && !with_c)) continue;
+      const T* src = (isc ? rowC : rowB) + (unsigned)forgotten(off[k]);
+      if (vbc == 2 && left >= TILE) {
+        v[k] = *reinterpret_cast<const V*>(src);
+      } else {
+        const int r = u0 - isc * HALF + lane, n = r % (NP / 4) * 4;
+        v[k] = V{};
+        if (r / (NP / 4) < left && n < a.N) {
+          if (vbc) {
+            v[k] = *reinterpret_cast<const V*>(src);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.N) v[k][e] = (float)src[e];
+            for (int e = 0; e < 4; ++e)
+              if (n + e < a.N) v[k][e] = src[e];
+          }
         }
       }
     }
   }
-  __device__ __forceinline__ void store(float* lds, int t0, int n) const {   // positions behind the end hold zeros, whatever was there
+  __device__ __forceinline__ void store(float* lds, int live, int w, int lane) {   // live: positions of the tile up to the end; behind it zeros, whatever was there
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int i = k * kWaves * 64 + (int)threadIdx.x, half = UNITS / 2, r = i >= half ? i - half : i;
-      const bool live = t0 + r / (NP / 4) < n;
-      if (i < UNITS) *reinterpret_cast<float4*>(lds + i * 4) = live ? make_float4(v[k][0], v[k][1], v[k][2], v[k][3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      const int u0 = (k * W + w) * 64, r = u0 - (u0 >= HALF) * HALF + lane;
+      float4 o = make_float4((float)v[k][0], (float)v[k][1], (float)v[k][2], (float)v[k][3]);
+      if (live < TILE && r / (NP / 4) >= live) o = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (u0 < 2 * HALF) *reinterpret_cast<float4*>(lds + (u0 + lane) * 4) = o;
     }
   }
 };
 
 // ------------------------------------------------------------------------------------------------------------------ forward
 // STATE: only the segment's end state (from zero) and its sum of delta
-template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds__(kWaves * 64) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
-  constexpr int CPL = FwdShape<NPL>::CPL, TT = FwdShape<NPL>::TT, TILE = kWaves * TT, NI = TT / 4, NP = 4 * NPL, CW = 16 * CPL;
-  constexpr int CK = kWaves * BwdShape<NPL>::TT;   // positions between the states that the backward starts from
+template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape<NPL>::W * 64) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
+  constexpr int W = FwdShape<NPL>::W, TT = FwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL;
+  constexpr int CK = BwdShape<NPL>::W * BwdShape<NPL>::TT;   // positions between the states that the backward starts from
   __shared__ float bc[2][TILE * NP * 2];
-  __shared__ float ex[kWaves][2][CPL][64 * NPL];
+  __shared__ float ex[W][2][64 * NPL];
+  __shared__ float carry[2][64 * NPL];   // the state in front of a tile, from the last wave of the tile before
   const Where at = where_of(a, p);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane & 3;
-  const int ch = at.cb * CW + (lane >> 2) * CPL, nch = p.dg - ch;   // channel within the group, how many from there on exist
-  const int chc = nch > 0 ? ch : (VCH ? p.dg - CPL : p.dg - 1), last = nch > 0 ? nch - 1 : (VCH ? CPL - 1 : 0), d = at.g * p.dg + chc;
+  const bool on = at.cb * 16 + (lane >> 2) < p.dg;   // (a channel that does not exist walks along on the group's last one and writes nothing)
+  const int ch = on ? at.cb * 16 + (lane >> 2) : p.dg - 1, dg0 = at.g * p.dg, d = dg0 + ch;
   const int n = mix_length(a.lengths, at.b, a.L), N = a.N, L = a.L;
-  float A[CPL][NPL], h[CPL][NPL], hc[CPL][NPL], bias[CPL], Dp[CPL];
+  const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
+  const bool gate = !STATE && a.z;
+  float A[NPL], hc[NPL];
 #pragma unroll
-  for (int c = 0; c < CPL; ++c) {
-    const int dc = d + (c < last ? c : last);
-    bias[c] = a.dt_bias ? a.dt_bias[dc] : 0.0f;
-    Dp[c] = a.Dp ? a.Dp[dc] : 0.0f;
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      const int s = q * NPL + j;
-      A[c][j] = s < N ? a.A[(int64_t)dc * N + s] * kLog2e : 0.0f;
-      hc[c][j] = !STATE && s < N && a.h0 ? a.h0[((int64_t)at.b * a.D + dc) * N + s] : 0.0f;
-    }
+  for (int j = 0; j < NPL; ++j) {
+    const int s = q * NPL + j;
+    A[j] = s < N ? a.A[(int64_t)d * N + s] * kLog2e : 0.0f;
+    hc[j] = !STATE && w == W - 1 && s < N && a.h0 ? a.h0[((int64_t)at.b * a.D + d) * N + s] : 0.0f;
+  }
+  if (w == W - 1) {
     if (!STATE)
       for (int k = 0; k < at.seg; ++k) {   // the segments in front
-        const int64_t r = ((int64_t)at.b * p.nseg + k) * a.D + dc;
+        const int64_t r = ((int64_t)at.b * p.nseg + k) * a.D + d;
         const float S = p.segs[r];
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) hc[c][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A[c][j] * S), hc[c][j], p.segh[r * NP + q * NPL + j]);
+        for (int j = 0; j < NPL; ++j) hc[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A[j] * S), hc[j], p.segh[r * NP + q * NPL + j]);
       }
+    mix_store<float, NPL>(&carry[0][lane * NPL], hc);
   }
-  const int dg0 = at.g * p.dg;   // uniform: the group's first channel
-  const T* pu = (const T*)a.u + at.b * a.su_b + dg0;
-  const T* pd = (const T*)a.dt + at.b * a.sdt_b + dg0;
-  const T* pz = a.z ? (const T*)a.z + at.b * a.sz_b + dg0 : nullptr;
-  const T* pB = (const T*)a.Bm + at.b * a.sB_b + at.g * a.sB_g;
-  const T* pC = (const T*)a.Cm + at.b * a.sC_b + at.g * a.sC_g;
-  T* py = (T*)a.y + (int64_t)at.b * L * a.D + dg0;
-  unsigned ou[CPL], od[CPL], oz[CPL], oy[CPL];
-  offsets<CPL>(ou, a.su_l, q, chc, last);
-  offsets<CPL>(od, a.sdt_l, q, chc, last);
-  offsets<CPL>(oz, a.sz_l, q, chc, last);
-  offsets<CPL>(oy, a.D, q, chc, last);
-  float ru[NI][CPL], rd[NI][CPL], rz[NI][CPL], Ssum[CPL];
-#pragma unroll
-  for (int c = 0; c < CPL; ++c) Ssum[c] = 0.0f;
-  StageBC<T, NP, TILE> st;
-  auto fetch = [&](int t0) {
-    const int tb = t0 + w * TT;
-    const bool whole = tb + TT <= L;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (whole || tb + 4 * i + q < L) {
-        load_ch<T, CPL, VCH>(pu + (int64_t)(tb + 4 * i) * a.su_l, ou, ru[i]);
-        load_ch<T, CPL, VCH>(pd + (int64_t)(tb + 4 * i) * a.sdt_l, od, rd[i]);
-        if (!STATE && pz) load_ch<T, CPL, VCH>(pz + (int64_t)(tb + 4 * i) * a.sz_l, oz, rz[i]);
-      }
-    st.load(a, p, pB, pC, t0, !STATE);
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, Dp = a.Dp ? a.Dp[d] : 0.0f;
+  const int t00 = k0 * TILE + w * TT;
+  Column<const T> cu, cd, cz;
+  Column<T> cy;
+  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, TILE, q, ch);
+  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, TILE, q, ch);
+  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, TILE, q, ch);
+  cy.start(a.y, (int64_t)L * a.D, a.D, at.b, dg0, t00, TILE, q, ch);
+  StageBC<T, NP, TILE, W> st;
+  st.start(a, at, k0 * TILE, TILE, w, lane);
+  T ru[NI], rd[NI], rz[NI];
+  float Ssum = 0.0f;
+  auto fetch = [&](int t0) {   // ... and on to the tile behind it
+    const int left = L - t0 - w * TT;
+    const bool whole = left >= TT;
+    get_all(cu, whole, left, q, ru);
+    get_all(cd, whole, left, q, rd);
+    if (gate) get_all(cz, whole, left, q, rz);
+    st.load(a, p.vbc, L - t0, !STATE, w, lane);
+    cu.move();
+    cd.move();
+    cz.move();
+    st.move();
   };
-  auto put = [&](int t0, const float (&v)[NI][CPL]) {
-    const int tb = t0 + w * TT;
-    const bool whole = tb + TT <= L;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (whole || tb + 4 * i + q < L) store_ch<T, CPL, VCH>(py + (int64_t)(tb + 4 * i) * a.D, oy, nch, v[i]);
-  };
-  const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
   if (k0 < k1 && k0 * TILE < n) fetch(k0 * TILE);
   for (int k = k0; k < k1; ++k) {
-    const int t0 = k * TILE;
+    const int t0 = k * TILE, par = (k - k0) & 1, tw = t0 + w * TT;
     if (t0 >= n) {   // (the whole workgroup) behind the end
       if (!STATE) {
-        const float zero[NI][CPL] = {};
-        put(t0, zero);
+        const float zero[NI] = {};
+        put_all(cy, L - tw >= TT, L - tw, q, on, zero);
+        cy.move();
       }
       continue;
     }
-    float u[NI][CPL], dl[NI][CPL], du[NI][CPL], z[NI][CPL], S[CPL];
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) S[c] = 0.0f;
+    float u[NI], dl[NI], du[NI], z[NI], S = 0.0f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const bool live = t0 + w * TT + 4 * i + q < n;
+      const float raw = (float)rd[i] + bias;
+      u[i] = (float)ru[i];
+      dl[i] = a.softplus ? mix_softplus(raw) : raw;
+      z[i] = (float)rz[i];
+    }
+    if (n - tw < TT) {
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const float raw = rd[i][c] + bias[c];
-        u[i][c] = live ? ru[i][c] : 0.0f;
-        dl[i][c] = live ? (a.softplus ? mix_softplus(raw) : raw) : 0.0f;
-        du[i][c] = dl[i][c] * u[i][c];
-        z[i][c] = rz[i][c];
-        S[c] += dl[i][c];
+      for (int i = 0; i < NI; ++i) {
+        const bool live = 4 * i + q < n - tw;
+        u[i] = live ? u[i] : 0.0f;
+        dl[i] = live ? dl[i] : 0.0f;
       }
     }
-    float* lds = bc[k & 1];
-    st.store(lds, t0, n);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      du[i] = dl[i] * u[i];
+      S += dl[i];
+    }
+    float* lds = bc[par];
+    st.store(lds, n - t0, w, lane);
     __syncthreads();
     if (k + 1 < k1 && t0 + TILE < n) fetch(t0 + TILE);
     const float* Bs = lds + w * TT * NP + q * NPL;
     const float* Cs = Bs + TILE * NP;
-    float dec[TT][CPL][NPL];
+    float dec[TT][NPL], h[NPL], e[NPL], P[NPL];
 #pragma unroll
-    for (int c = 0; c < CPL; ++c)
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) h[c][j] = 0.0f;
+    for (int j = 0; j < NPL; ++j) e[j] = 0.0f;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       float Bv[NPL];
       mix_load<float, NPL>(Bs + t * NP, Bv);
+      const float dt = quad_bcast(dl[t / 4], t & 3), x = quad_bcast(du[t / 4], t & 3);
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const float dt = quad_bcast(dl[t / 4][c], t & 3), x = quad_bcast(du[t / 4][c], t & 3);
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-          dec[t][c][j] = __builtin_amdgcn_exp2f(dt * A[c][j]);
-          h[c][j] = __builtin_fmaf(dec[t][c][j], h[c][j], x * Bv[j]);
-        }
+      for (int j = 0; j < NPL; ++j) {
+        dec[t][j] = __builtin_amdgcn_exp2f(dt * A[j]);
+        e[j] = __builtin_fmaf(dec[t][j], e[j], x * Bv[j]);
       }
     }
+    S = quad_sum(S);
+    Ssum += S;
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      S[c] = quad_sum(S[c]);
-      Ssum[c] += S[c];
-      float P[NPL];
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) P[j] = __builtin_amdgcn_exp2f(A[c][j] * S[c]);
-      mix_store<float, NPL>(&ex[w][0][c][lane * NPL], h[c]);
-      mix_store<float, NPL>(&ex[w][1][c][lane * NPL], P);
-    }
+    for (int j = 0; j < NPL; ++j) P[j] = __builtin_amdgcn_exp2f(A[j] * S);
+    mix_store<float, NPL>(&ex[w][0][lane * NPL], e);
+    mix_store<float, NPL>(&ex[w][1][lane * NPL], P);
     __syncthreads();
+    // h: the state in front of this wave's positions; the last wave goes on to the next tile's
+    mix_load<float, NPL>(&carry[par][lane * NPL], h);
+#pragma unroll(NPL < 8 ? 4 : NPL < 16 ? 2 : 1)
+    for (int v = 0; v < w; ++v) {
+      float x[NPL], y[NPL];
+      mix_load<float, NPL>(&ex[v][0][lane * NPL], x);
+      mix_load<float, NPL>(&ex[v][1][lane * NPL], y);
 #pragma unroll
-    for (int v = 0; v < kWaves; ++v) {   // h: this wave's initial state, hc: the next tile's
-      if (v == w) {
+      for (int j = 0; j < NPL; ++j) h[j] = __builtin_fmaf(y[j], h[j], x[j]);
+    }
+    if (w == W - 1) {
 #pragma unroll
-        for (int c = 0; c < CPL; ++c)
-#pragma unroll
-          for (int j = 0; j < NPL; ++j) h[c][j] = hc[c][j];
-      }
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        float e[NPL], P[NPL];
-        mix_load<float, NPL>(&ex[v][0][c][lane * NPL], e);
-        mix_load<float, NPL>(&ex[v][1][c][lane * NPL], P);
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) hc[c][j] = __builtin_fmaf(P[j], hc[c][j], e[j]);
-      }
+      for (int j = 0; j < NPL; ++j) hc[j] = __builtin_fmaf(P[j], h[j], e[j]);
+      mix_store<float, NPL>(&carry[par ^ 1][lane * NPL], hc);
     }
     if constexpr (!STATE) {
-      if (a.ckpt && (w * TT) % CK == 0 && t0 + w * TT < n) {
-        const int64_t r = ((int64_t)at.b * p.nck + (t0 + w * TT) / CK) * a.D + d;
-#pragma unroll
-        for (int c = 0; c < CPL; ++c)
-          if (c < nch) mix_store<float, NPL>(a.ckpt + (r + c) * NP + q * NPL, h[c]);
-      }
-      float y[NI][CPL];
+      if (a.ckpt && (w * TT) % CK == 0 && tw < n && on)
+        mix_store<float, NPL>(a.ckpt + (((int64_t)at.b * p.nck + tw / CK) * a.D + dg0) * NP + (unsigned)(ch * NP + q * NPL), h);
+      float y[NI];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        float Bv[NPL], Cv[NPL];
+        float Bv[NPL], Cv[NPL], s = 0.0f;
         mix_load<float, NPL>(Bs + t * NP, Bv);
         mix_load<float, NPL>(Cs + t * NP, Cv);
+        const float x = quad_bcast(du[t / 4], t & 3);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const float x = quad_bcast(du[t / 4][c], t & 3);
-          float s = 0.0f;
-#pragma unroll
-          for (int j = 0; j < NPL; ++j) {
-            h[c][j] = __builtin_fmaf(dec[t][c][j], h[c][j], x * Bv[j]);
-            s = __builtin_fmaf(Cv[j], h[c][j], s);
-          }
-          s = quad_sum(s);
-          y[t / 4][c] = (t & 3) == 0 || q == (t & 3) ? s : y[t / 4][c];
+        for (int j = 0; j < NPL; ++j) {
+          h[j] = __builtin_fmaf(dec[t][j], h[j], x * Bv[j]);
+          s = __builtin_fmaf(Cv[j], h[j], s);
         }
+        s = quad_sum(s);
+        y[t / 4] = (t & 3) == 0 || q == (t & 3) ? s : y[t / 4];
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int t = t0 + w * TT + 4 * i + q;
+      for (int i = 0; i < NI; ++i) y[i] = __builtin_fmaf(Dp, u[i], y[i]);
+      if (gate) {
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          y[i][c] = __builtin_fmaf(Dp[c], u[i][c], y[i][c]);
-          if (pz) y[i][c] *= z[i][c] * mix_sigmoid(z[i][c]);
-          if (t >= n) y[i][c] = 0.0f;
-        }
+        for (int i = 0; i < NI; ++i) y[i] *= z[i] * mix_sigmoid(z[i]);
       }
-      put(t0, y);
+      if (n - tw < TT) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) y[i] = 4 * i + q < n - tw ? y[i] : 0.0f;
+      }
+      put_all(cy, L - tw >= TT, L - tw, q, on, y);
+      cy.move();
     }
   }
   if constexpr (STATE) {
     __syncthreads();
-    float* red = &ex[0][0][0][0];   // [wave][channel]
-    if (q == 0)
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) red[w * CW + (lane >> 2) * CPL + c] = Ssum[c];
+    float* red = &ex[0][0][0];   // [wave][channel]
+    if (q == 0) red[w * 16 + (lane >> 2)] = Ssum;
     __syncthreads();
-    if (w == 0) {
+    if (w == W - 1 && on) {
       const int64_t r = ((int64_t)at.b * p.nseg + at.seg) * a.D + d;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (c < nch) {
-          float S = 0.0f;
-          for (int v = 0; v < kWaves; ++v) S += red[v * CW + (lane >> 2) * CPL + c];
-          if (q == 0) p.segs[r + c] = S;
-          mix_store<float, NPL>(p.segh + (r + c) * NP + q * NPL, hc[c]);
-        }
+      float S = 0.0f;
+      for (int v = 0; v < W; ++v) S += red[v * 16 + (lane >> 2)];
+      if (q == 0) p.segs[r] = S;
+      mix_store<float, NPL>(p.segh + r * NP + q * NPL, hc);
     }
-  } else if (a.h_out && at.seg == p.nseg - 1 && w == 0) {
+  } else if (a.h_out && at.seg == p.nseg - 1 && w == W - 1 && on) {
 #pragma unroll
-    for (int c = 0; c < CPL; ++c)
-#pragma unroll
-      for (int j = 0; j < NPL; ++j)
-        if (c < nch && q * NPL + j < N) a.h_out[((int64_t)at.b * a.D + d + c) * N + q * NPL + j] = hc[c][j];
+    for (int j = 0; j < NPL; ++j)
+      if (q * NPL + j < N) a.h_out[((int64_t)at.b * a.D + d) * N + q * NPL + j] = hc[j];
   }
 }
 
@@ -373,138 +384,134 @@ template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds_
 // With e_t = a_t G_t, G_t = C_t gy'_t + e_{t+1} (gy' = gy silu(z)): du = delta sum_n G B + D gy', ddelta = sum_n e h_{t-1} A + u sum_n G B, dA = sum_t e h_{t-1} delta,
 // dB = sum_channels G delta u, dC = sum_channels gy' h.  Tiles from the sequence's end; inside a tile the waves first walk both ways from zero (forward
 // for h, backward for e), meet in LDS, and walk both ways again from the right ends, the states of the second walk staying in registers.  dB and dC are
-// summed over the 32 (16) channels of a workgroup by lane exchanges and over workgroups from `part_bc`; everything in a fixed order.
+// summed over the 16 channels of a workgroup by lane exchanges and over workgroups from `part_bc`; everything in a fixed order.
 // STATE: only e at the segment's start (from zero) and the sum of delta.
-template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds__(kWaves * 64) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
-  constexpr int CPL = BwdShape<NPL>::CPL, TT = BwdShape<NPL>::TT, TILE = kWaves * TT, NI = TT / 4, NP = 4 * NPL, CW = 16 * CPL, NX = STATE ? 2 : 3;
+template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape<NPL>::W * 64) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
+  constexpr int W = BwdShape<NPL>::W, TT = BwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL, NX = STATE ? 2 : 3;
   __shared__ float bc[2][TILE * NP * 2];
-  __shared__ float ex[kWaves][NX][CPL][64 * NPL];
+  __shared__ float ex[W][NX][64 * NPL];
+  __shared__ float carry[2][64 * NPL];   // e in front of a tile, from the first wave of the tile behind
   const Where at = where_of(a, p);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), q = lane & 3;
-  const int ch = at.cb * CW + (lane >> 2) * CPL, nch = p.dg - ch;
-  const int chc = nch > 0 ? ch : (VCH ? p.dg - CPL : p.dg - 1), last = nch > 0 ? nch - 1 : (VCH ? CPL - 1 : 0), d = at.g * p.dg + chc;
+  const bool on = at.cb * 16 + (lane >> 2) < p.dg;   // (a channel that does not exist has a gradient of zero, so that it adds nothing to dB and dC)
+  const int ch = on ? at.cb * 16 + (lane >> 2) : p.dg - 1, dg0 = at.g * p.dg, d = dg0 + ch;
   const int n = mix_length(a.lengths, at.b, a.L), N = a.N, L = a.L;
-  float A[CPL][NPL], ec[CPL][NPL], gA[CPL][NPL], bias[CPL], Dp[CPL], gD[CPL], gb[CPL], Ssum[CPL];
+  const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
+  const bool gate = a.z != nullptr, has_gy = a.gy != nullptr;
+  float A[NPL], ec[NPL], gA[NPL], gD = 0.0f, gb = 0.0f, Ssum = 0.0f;
 #pragma unroll
-  for (int c = 0; c < CPL; ++c) {
-    const int dc = d + (c < last ? c : last);
-    bias[c] = a.dt_bias ? a.dt_bias[dc] : 0.0f;
-    Dp[c] = a.Dp ? a.Dp[dc] : 0.0f;
-    gD[c] = gb[c] = Ssum[c] = 0.0f;
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) {
-      const int s = q * NPL + j;
-      A[c][j] = s < N ? a.A[(int64_t)dc * N + s] * kLog2e : 0.0f;
-      ec[c][j] = !STATE && c < nch && s < N && a.gh ? a.gh[((int64_t)at.b * a.D + dc) * N + s] : 0.0f;   // (a channel that is not there adds nothing to dB)
-      gA[c][j] = 0.0f;
-    }
-    if (!STATE && c < nch)
+  for (int j = 0; j < NPL; ++j) {
+    const int s = q * NPL + j;
+    A[j] = s < N ? a.A[(int64_t)d * N + s] * kLog2e : 0.0f;
+    ec[j] = !STATE && w == 0 && on && s < N && a.gh ? a.gh[((int64_t)at.b * a.D + d) * N + s] : 0.0f;
+    gA[j] = 0.0f;
+  }
+  if (w == 0) {
+    if (!STATE && on)
       for (int k = p.nseg - 1; k > at.seg; --k) {   // the segments behind
-        const int64_t r = ((int64_t)at.b * p.nseg + k) * a.D + dc;
+        const int64_t r = ((int64_t)at.b * p.nseg + k) * a.D + d;
         const float S = p.segs[r];
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) ec[c][j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A[c][j] * S), ec[c][j], p.segh[r * NP + q * NPL + j]);
+        for (int j = 0; j < NPL; ++j) ec[j] = __builtin_fmaf(__builtin_amdgcn_exp2f(A[j] * S), ec[j], p.segh[r * NP + q * NPL + j]);
       }
+    mix_store<float, NPL>(&carry[0][lane * NPL], ec);
   }
-  const int dg0 = at.g * p.dg;   // uniform: the group's first channel
-  const T* pu = (const T*)a.u + at.b * a.su_b + dg0;
-  const T* pd = (const T*)a.dt + at.b * a.sdt_b + dg0;
-  const T* pz = a.z ? (const T*)a.z + at.b * a.sz_b + dg0 : nullptr;
-  const T* pg = a.gy ? (const T*)a.gy + at.b * a.sg_b + dg0 : nullptr;
-  const T* pB = (const T*)a.Bm + at.b * a.sB_b + at.g * a.sB_g;
-  const T* pC = (const T*)a.Cm + at.b * a.sC_b + at.g * a.sC_g;
-  const int64_t o0 = (int64_t)at.b * L * a.D + dg0;
-  unsigned ou[CPL], od[CPL], oz[CPL], og[CPL], oo[CPL];
-  offsets<CPL>(ou, a.su_l, q, chc, last);
-  offsets<CPL>(od, a.sdt_l, q, chc, last);
-  offsets<CPL>(oz, a.sz_l, q, chc, last);
-  offsets<CPL>(og, a.sg_l, q, chc, last);
-  offsets<CPL>(oo, a.D, q, chc, last);
-  float ru[NI][CPL], rd[NI][CPL], rz[NI][CPL], rg[NI][CPL];
-  StageBC<T, NP, TILE> st;
-  auto fetch = [&](int t0) {
-    const int tb = t0 + w * TT;
-    const bool whole = tb + TT <= L;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (whole || tb + 4 * i + q < L) {
-        if (!STATE) load_ch<T, CPL, VCH>(pu + (int64_t)(tb + 4 * i) * a.su_l, ou, ru[i]);
-        load_ch<T, CPL, VCH>(pd + (int64_t)(tb + 4 * i) * a.sdt_l, od, rd[i]);
-        if (pz) load_ch<T, CPL, VCH>(pz + (int64_t)(tb + 4 * i) * a.sz_l, oz, rz[i]);
-        if (pg) load_ch<T, CPL, VCH>(pg + (int64_t)(tb + 4 * i) * a.sg_l, og, rg[i]);
-      }
-    st.load(a, p, pB, pC, t0, true);
-  };
-  auto put = [&](void* to, int t0, const float (&v)[NI][CPL]) {
-    const int tb = t0 + w * TT;
-    const bool whole = tb + TT <= L;
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      if (whole || tb + 4 * i + q < L) store_ch<T, CPL, VCH>((T*)to + o0 + (int64_t)(tb + 4 * i) * a.D, oo, nch, v[i]);
-  };
-  const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.0f, Dp = a.Dp ? a.Dp[d] : 0.0f;
   int kl = k1;   // tiles from kl on lie behind the end
   while (kl > k0 && (kl - 1) * TILE >= n) --kl;
+  const int64_t LD = (int64_t)L * a.D;
   if (!STATE)
     for (int k = kl; k < k1; ++k) {
-      const float zero[NI][CPL] = {};
-      put(a.gu, k * TILE, zero);
-      put(a.gdt, k * TILE, zero);
-      if (pz) put(a.gz, k * TILE, zero);
+      const int tw = k * TILE + w * TT;
+      const float zero[NI] = {};
+      Column<T> c;
+      c.start(a.gu, LD, a.D, at.b, dg0, tw, 0, q, ch);
+      put_all(c, false, L - tw, q, on, zero);
+      c.start(a.gdt, LD, a.D, at.b, dg0, tw, 0, q, ch);
+      put_all(c, false, L - tw, q, on, zero);
+      c.start(a.gz, LD, a.D, at.b, dg0, tw, 0, q, ch);
+      if (gate) put_all(c, false, L - tw, q, on, zero);
     }
+  const int t00 = (kl - 1) * TILE + w * TT;
+  Column<const T> cu, cd, cz, cg;
+  Column<T> co;   // one row pointer for the three outputs, which are alike: gdt and gz at fixed distances
+  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, -TILE, q, ch);
+  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, -TILE, q, ch);
+  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, -TILE, q, ch);
+  cg.start(a.gy, a.sg_b, a.sg_l, at.b, dg0, t00, -TILE, q, ch);
+  co.start(a.gu, LD, a.D, at.b, dg0, t00, -TILE, q, ch);
+  StageBC<T, NP, TILE, W> st;
+  st.start(a, at, (kl - 1) * TILE, -TILE, w, lane);
+  T ru[NI], rd[NI], rz[NI], rg[NI];
+  auto fetch = [&](int t0) {   // ... and on to the tile in front of it
+    const int left = L - t0 - w * TT;
+    const bool whole = left >= TT;
+    if (!STATE) get_all(cu, whole, left, q, ru);
+    get_all(cd, whole, left, q, rd);
+    if (gate) get_all(cz, whole, left, q, rz);
+    if (has_gy) get_all(cg, whole, left, q, rg);
+    st.load(a, p.vbc, L - t0, true, w, lane);
+    cu.move();
+    cd.move();
+    cz.move();
+    cg.move();
+    st.move();
+  };
+  // where a lane leaves its share of dB and dC (the walk's reduction below)
+  const unsigned out_off = NPL < 4 ? ((lane >> 4) & 1) * NP + q * NPL + (lane >> 5) : (lane & 4 ? NP : 0) + q * NPL + ((lane >> 4) & 1) * 2 + (lane >> 5);
+  const bool out_on = NPL < 4 ? (lane & 12) == 0 : (lane & 8) == 0;
   if (kl > k0) fetch((kl - 1) * TILE);
   for (int k = kl - 1; k >= k0; --k) {
-    const int t0 = k * TILE;
-    float u[NI][CPL], dl[NI][CPL], du[NI][CPL], raw[NI][CPL], gp[NI][CPL], gy[NI][CPL], z[NI][CPL], S[CPL], hi[CPL][NPL];
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) S[c] = 0.0f;
+    const int t0 = k * TILE, par = (kl - 1 - k) & 1, tw = t0 + w * TT;
+    float u[NI], dl[NI], du[NI], raw[NI], gp[NI], gy[NI], z[NI], S = 0.0f, hi[NPL];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int t = t0 + w * TT + 4 * i + q;
+      raw[i] = (float)rd[i] + bias;
+      u[i] = STATE ? 0.0f : (float)ru[i];
+      dl[i] = a.softplus ? mix_softplus(raw[i]) : raw[i];
+      gy[i] = has_gy ? (float)rg[i] : 0.0f;
+      z[i] = (float)rz[i];
+    }
+    if (n - tw < TT || !on) {
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const bool live = t < n && c < nch;
-        raw[i][c] = rd[i][c] + bias[c];
-        u[i][c] = !STATE && live ? ru[i][c] : 0.0f;
-        dl[i][c] = live ? (a.softplus ? mix_softplus(raw[i][c]) : raw[i][c]) : 0.0f;
-        du[i][c] = dl[i][c] * u[i][c];
-        gy[i][c] = pg && live ? rg[i][c] : 0.0f;
-        z[i][c] = rz[i][c];
-        gp[i][c] = pz ? (live ? gy[i][c] * z[i][c] * mix_sigmoid(z[i][c]) : 0.0f) : gy[i][c];
-        S[c] += dl[i][c];
+      for (int i = 0; i < NI; ++i) {
+        const bool live = 4 * i + q < n - tw && on;
+        u[i] = live ? u[i] : 0.0f;
+        dl[i] = live ? dl[i] : 0.0f;
+        gy[i] = live ? gy[i] : 0.0f;
+        z[i] = live ? z[i] : 0.0f;
+        raw[i] = live ? raw[i] : 0.0f;
       }
     }
-    float* lds = bc[k & 1];
-    st.store(lds, t0, n);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      du[i] = dl[i] * u[i];
+      gp[i] = gate ? gy[i] * z[i] * mix_sigmoid(z[i]) : gy[i];
+      S += dl[i];
+    }
+    float* lds = bc[par];
+    st.store(lds, n - t0, w, lane);
     __syncthreads();
     if (STATE && k > k0) fetch(t0 - TILE);
-    if constexpr (!STATE) {
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) mix_load<float, NPL>(a.ckpt + (((int64_t)at.b * p.nck + k) * a.D + dg0) * NP + (unsigned)forgotten((chc + (c < last ? c : last)) * NP + q * NPL), hi[c]);
-    }
+    if constexpr (!STATE) mix_load<float, NPL>(a.ckpt + (((int64_t)at.b * p.nck + k) * a.D + dg0) * NP + (unsigned)forgotten(ch * NP + q * NPL), hi);
     const float* Bs = lds + forgotten(w * TT * NP + q * NPL);
     const float* Cs = Bs + TILE * NP;
     // (with 16 states a lane the decays do not fit beside the walk's own values: they are computed again wherever they are used)
     constexpr bool KEEP = STATE || NPL < 16;
-    float dec[TT][CPL][NPL], e[CPL][NPL], h[CPL][NPL];
-    auto decay = [&](int t, int c, int j, float dt) { return KEEP ? dec[t][c][j] : __builtin_amdgcn_exp2f(dt * A[c][j]); };
+    float dec[TT][NPL], e[NPL], h[NPL], P[NPL], own[NPL];
+    auto decay = [&](int t, int j, float dt) { return KEEP ? dec[t][j] : __builtin_amdgcn_exp2f(dt * A[j]); };
 #pragma unroll
-    for (int c = 0; c < CPL; ++c)
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) h[c][j] = e[c][j] = 0.0f;
+    for (int j = 0; j < NPL; ++j) h[j] = own[j] = 0.0f;
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       float Bv[NPL];
       if (!STATE) mix_load<float, NPL>(Bs + t * NP, Bv);
+      const float dt = quad_bcast(dl[t / 4], t & 3), x = quad_bcast(du[t / 4], t & 3);
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const float dt = quad_bcast(dl[t / 4][c], t & 3), x = quad_bcast(du[t / 4][c], t & 3);
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-          const float f = __builtin_amdgcn_exp2f(dt * A[c][j]);
-          if (KEEP) dec[t][c][j] = f;
-          if (!STATE) h[c][j] = __builtin_fmaf(f, h[c][j], x * Bv[j]);
-        }
+      for (int j = 0; j < NPL; ++j) {
+        const float f = __builtin_amdgcn_exp2f(dt * A[j]);
+        if (KEEP) dec[t][j] = f;
+        if (!STATE) h[j] = __builtin_fmaf(f, h[j], x * Bv[j]);
       }
       if (!KEEP) __builtin_amdgcn_sched_barrier(0);   // (registers, not overlap, are short)
     }
@@ -516,71 +523,58 @@ template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds_
     for (int t = TT - 1; t >= 0; --t) {
       float Cv[NPL];
       mix_load<float, NPL>(Cs + t * NP, Cv);
+      const float g = quad_bcast(gp[t / 4], t & 3), dt = quad_bcast(dl[t / 4], t & 3);
 #pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        const float g = quad_bcast(gp[t / 4][c], t & 3), dt = quad_bcast(dl[t / 4][c], t & 3);
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) e[c][j] = decay(t, c, j, dt) * __builtin_fmaf(Cv[j], g, e[c][j]);
-      }
+      for (int j = 0; j < NPL; ++j) own[j] = decay(t, j, dt) * __builtin_fmaf(Cv[j], g, own[j]);
       if (!KEEP) __builtin_amdgcn_sched_barrier(0);
     }
+    S = quad_sum(S);
+    Ssum += S;
 #pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      S[c] = quad_sum(S[c]);
-      Ssum[c] += S[c];
-      float P[NPL];
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) P[j] = __builtin_amdgcn_exp2f(A[c][j] * S[c]);
-      mix_store<float, NPL>(&ex[w][0][c][lane * NPL], P);
-      mix_store<float, NPL>(&ex[w][1][c][lane * NPL], e[c]);
-      if constexpr (!STATE) mix_store<float, NPL>(&ex[w][NX - 1][c][lane * NPL], h[c]);
-    }
+    for (int j = 0; j < NPL; ++j) P[j] = __builtin_amdgcn_exp2f(A[j] * S);
+    mix_store<float, NPL>(&ex[w][0][lane * NPL], P);
+    mix_store<float, NPL>(&ex[w][1][lane * NPL], own);
+    if constexpr (!STATE) mix_store<float, NPL>(&ex[w][NX - 1][lane * NPL], h);
     __syncthreads();
-#pragma unroll(NPL < 16 ? 2 : 1)
-    for (int v = kWaves - 1; v >= 0; --v) {   // e: what arrives behind this wave's positions, ec: behind the next tile's
-      if (v == w) {
+    // e: what arrives behind this wave's positions; the first wave goes on to what arrives behind the next tile
+    mix_load<float, NPL>(&carry[par][lane * NPL], e);
+#pragma unroll(NPL < 8 ? 4 : NPL < 16 ? 2 : 1)
+    for (int v = W - 1; v > w; --v) {
+      float x[NPL], y[NPL];
+      mix_load<float, NPL>(&ex[v][0][lane * NPL], y);
+      mix_load<float, NPL>(&ex[v][1][lane * NPL], x);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c)
+      for (int j = 0; j < NPL; ++j) e[j] = __builtin_fmaf(y[j], e[j], x[j]);
+    }
+    if (w == 0) {
 #pragma unroll
-          for (int j = 0; j < NPL; ++j) e[c][j] = ec[c][j];
-      }
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) {
-        float x[NPL], P[NPL];
-        mix_load<float, NPL>(&ex[v][0][c][lane * NPL], P);
-        mix_load<float, NPL>(&ex[v][1][c][lane * NPL], x);
-#pragma unroll
-        for (int j = 0; j < NPL; ++j) ec[c][j] = __builtin_fmaf(P[j], ec[c][j], x[j]);
-      }
+      for (int j = 0; j < NPL; ++j) ec[j] = __builtin_fmaf(P[j], e[j], own[j]);
+      mix_store<float, NPL>(&carry[par ^ 1][lane * NPL], ec);
     }
     if constexpr (!STATE) {
-#pragma unroll(NPL < 16 ? 2 : 1)
-      for (int v = 0; v < w; ++v)
+#pragma unroll(NPL < 8 ? 4 : NPL < 16 ? 2 : 1)
+      for (int v = 0; v < w; ++v) {
+        float x[NPL], y[NPL];
+        mix_load<float, NPL>(&ex[v][0][lane * NPL], y);
+        mix_load<float, NPL>(&ex[v][NX - 1][lane * NPL], x);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          float x[NPL], P[NPL];
-          mix_load<float, NPL>(&ex[v][0][c][lane * NPL], P);
-          mix_load<float, NPL>(&ex[v][NX - 1][c][lane * NPL], x);
-#pragma unroll
-          for (int j = 0; j < NPL; ++j) hi[c][j] = __builtin_fmaf(P[j], hi[c][j], x[j]);
-        }
+        for (int j = 0; j < NPL; ++j) hi[j] = __builtin_fmaf(y[j], hi[j], x[j]);
+      }
       // The second walk in parts of HALF positions from the last part to the first, so that only a part's states are in registers; h first reaches a
       // part's start without keeping any.
-      constexpr int HALF = NPL == 4 ? TT : NPL == 2 ? TT / 2 : NPL == 8 ? 2 : 1, PARTS = TT / HALF, JB = NPL < 4 ? NPL : 4;
-      float oB[NI][CPL], oG[NI][CPL], oY[NI][CPL];
+      constexpr int HALF = NPL <= 4 ? TT : NPL == 8 ? 2 : 1, PARTS = TT / HALF, JB = NPL < 4 ? NPL : 4;
+      float oB[NI], oG[NI], oY[NI];
       forget(gp);
       if (!KEEP) forget(A);
-      auto forward = [&](const float (*x)[NPL], int t, float (*to)[NPL]) {
+      auto forward = [&](const float* x, int t, float* to) {
         float Bv[NPL];
         mix_load<float, NPL>(Bs + t * NP, Bv);
+        const float v = quad_bcast(du[t / 4], t & 3), dt = quad_bcast(dl[t / 4], t & 3);
 #pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          const float v = quad_bcast(du[t / 4][c], t & 3), dt = quad_bcast(dl[t / 4][c], t & 3);
-#pragma unroll
-          for (int j = 0; j < NPL; ++j) to[c][j] = __builtin_fmaf(decay(t, c, j, dt), x[c][j], v * Bv[j]);
-        }
+        for (int j = 0; j < NPL; ++j) to[j] = __builtin_fmaf(decay(t, j, dt), x[j], v * Bv[j]);
         if (!KEEP) __builtin_amdgcn_sched_barrier(0);
       };
+      float* out = p.part_bc + ((((int64_t)at.cb * a.B + at.b) * L + tw) * a.G + at.g) * 2 * NP;   // (written where the position exists only)
 #pragma unroll
       for (int part = PARTS - 1; part >= 0; --part) {
         __builtin_amdgcn_sched_barrier(0);
@@ -591,7 +585,7 @@ template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds_
         Bs = lds + forgotten(w * TT * NP + q * NPL);
 #pragma unroll
         for (int t = 0; t < part * HALF; ++t) forward(t ? h : hi, t, h);
-        float hs[HALF][CPL][NPL];
+        float hs[HALF][NPL];
 #pragma unroll
         for (int t = 0; t < HALF; ++t) forward(t ? hs[t ? t - 1 : 0] : (part ? h : hi), part * HALF + t, hs[t]);
         forget(du);
@@ -601,128 +595,110 @@ template <typename T, int NPL, bool STATE, bool VCH> __global__ __launch_bounds_
 #pragma unroll
         for (int t = part * HALF + HALF - 1; t >= part * HALF; --t) {
           const int th = t - part * HALF;
-          const int tt = t0 + w * TT + t;
-          float* out = p.part_bc + ((((int64_t)at.cb * a.B + at.b) * L + tt) * a.G + at.g) * 2 * NP;   // (written where tt < n only)
-          float sB[CPL], sG[CPL], sY[CPL];
+          float* row = out + (int64_t)t * a.G * 2 * NP;
+          float sB = 0.0f, sG = 0.0f, sY = 0.0f;
+          const float g = quad_bcast(gp[t / 4], t & 3), x = quad_bcast(du[t / 4], t & 3), dt = quad_bcast(dl[t / 4], t & 3);
 #pragma unroll
           for (int j0 = 0; j0 < NPL; j0 += JB) {
             float Bv[JB], Cv[JB], pb[JB], pc[JB];
             mix_load<float, JB>(Bs + t * NP + j0, Bv);
             mix_load<float, JB>(Cs + t * NP + j0, Cv);
 #pragma unroll
-            for (int c = 0; c < CPL; ++c) {
-              const float g = quad_bcast(gp[t / 4][c], t & 3), x = quad_bcast(du[t / 4][c], t & 3), dt = quad_bcast(dl[t / 4][c], t & 3);
-              if (j0 == 0) sB[c] = sG[c] = sY[c] = 0.0f;
-#pragma unroll
-              for (int jj = 0; jj < JB; ++jj) {
-                const int j = j0 + jj;
-                const float ht = hs[th][c][j];
-                const float G = __builtin_fmaf(Cv[jj], g, e[c][j]);
-                e[c][j] = decay(t, c, j, dt) * G;
-                const float eh = e[c][j] * (th ? hs[th ? th - 1 : 0][c][j] : part ? h[c][j] : hi[c][j]);
-                gA[c][j] = __builtin_fmaf(eh, dt, gA[c][j]);
-                sG[c] = __builtin_fmaf(eh, A[c][j], sG[c]);
-                sB[c] = __builtin_fmaf(G, Bv[jj], sB[c]);
-                sY[c] = __builtin_fmaf(Cv[jj], ht, sY[c]);
-                pb[jj] = c ? __builtin_fmaf(G, x, pb[jj]) : G * x;
-                pc[jj] = c ? __builtin_fmaf(g, ht, pc[jj]) : g * ht;
-              }
+            for (int jj = 0; jj < JB; ++jj) {
+              const int j = j0 + jj;
+              const float ht = hs[th][j];
+              const float G = __builtin_fmaf(Cv[jj], g, e[j]);
+              e[j] = decay(t, j, dt) * G;
+              const float eh = e[j] * (th ? hs[th ? th - 1 : 0][j] : part ? h[j] : hi[j]);
+              gA[j] = __builtin_fmaf(eh, dt, gA[j]);
+              sG = __builtin_fmaf(eh, A[j], sG);
+              sB = __builtin_fmaf(G, Bv[jj], sB);
+              sY = __builtin_fmaf(Cv[jj], ht, sY);
+              pb[jj] = G * x;
+              pc[jj] = g * ht;
             }
             // sums over the 16 quads; the states of dB and of dC end up spread over the rows of 16 lanes
+            float v;
             if constexpr (JB == 4) {
               const float sb = sum_quads_of_row(fold16(fold32(pb[0], pb[1]), fold32(pb[2], pb[3])));
               const float sc = sum_quads_of_row(fold16(fold32(pc[0], pc[1]), fold32(pc[2], pc[3])));
-              const int s = q * NPL + j0 + ((lane >> 4) & 1) * 2 + (lane >> 5);
-              if ((lane & 8) == 0 && tt < n) out[(unsigned)forgotten((lane & 4 ? NP : 0) + s)] = lane & 4 ? sc : sb;
+              v = lane & 4 ? sc : sb;
             } else {
-              const float sv = sum_quads_of_row(fold16(fold32(pb[0], pb[1]), fold32(pc[0], pc[1])));
-              if ((lane & 12) == 0 && tt < n) out[(unsigned)forgotten(((lane >> 4) & 1) * NP + q * NPL + (lane >> 5))] = sv;
+              v = sum_quads_of_row(fold16(fold32(pb[0], pb[1]), fold32(pc[0], pc[1])));
             }
+            if (out_on && t < n - tw) (row + j0)[(unsigned)forgotten(out_off)] = v;
           }
           const bool mine = q == (t & 3) || (t & 3) == 3;   // (the highest of a lane's four comes first; the others then choose)
-#pragma unroll
-          for (int c = 0; c < CPL; ++c) {
-            const float vB = quad_sum(sB[c]), vG = quad_sum(sG[c]), vY = pz ? quad_sum(sY[c]) : 0.0f;
-            oB[t / 4][c] = mine ? vB : oB[t / 4][c];
-            oG[t / 4][c] = mine ? vG : oG[t / 4][c];
-            oY[t / 4][c] = mine ? vY : oY[t / 4][c];
-          }
+          const float vB = quad_sum(sB), vG = quad_sum(sG), vY = gate ? quad_sum(sY) : 0.0f;
+          oB[t / 4] = mine ? vB : oB[t / 4];
+          oG[t / 4] = mine ? vG : oG[t / 4];
+          oY[t / 4] = mine ? vY : oY[t / 4];
           __builtin_amdgcn_sched_barrier(0);
         }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const bool live = t0 + w * TT + 4 * i + q < n;
-#pragma unroll
-        for (int c = 0; c < CPL; ++c) {
-          float gd = __builtin_fmaf(kLn2, oG[i][c], u[i][c] * oB[i][c]);
-          if (a.softplus) gd *= mix_sigmoid(raw[i][c]);
-          oG[i][c] = live ? gd : 0.0f;
-          oB[i][c] = live ? __builtin_fmaf(dl[i][c], oB[i][c], Dp[c] * gp[i][c]) : 0.0f;
-          gD[c] = __builtin_fmaf(gp[i][c], u[i][c], gD[c]);
-          gb[c] += oG[i][c];
-          if (pz) {
-            const float s = mix_sigmoid(z[i][c]), yp = __builtin_fmaf(Dp[c], u[i][c], oY[i][c]);
-            oY[i][c] = live ? gy[i][c] * yp * s * (1.0f + z[i][c] * (1.0f - s)) : 0.0f;
-          }
+      for (int i = 0; i < NI; ++i) {   // (behind the end u, delta, gy, z and G are zero, and so is all of this but the sigmoid's factor)
+        float gd = __builtin_fmaf(kLn2, oG[i], u[i] * oB[i]);
+        if (a.softplus) gd *= mix_sigmoid(raw[i]);
+        const bool live = 4 * i + q < n - tw;
+        oG[i] = live ? gd : 0.0f;
+        const float gu = live ? __builtin_fmaf(dl[i], oB[i], Dp * gp[i]) : 0.0f;
+        gD = __builtin_fmaf(gp[i], u[i], gD);
+        gb += oG[i];
+        if (gate) {
+          const float s = mix_sigmoid(z[i]);
+          oY[i] = gy[i] * __builtin_fmaf(Dp, u[i], oY[i]) * s * (1.0f + z[i] * (1.0f - s));
         }
+        oB[i] = gu;
       }
-      put(a.gu, t0, oB);
-      put(a.gdt, t0, oG);
-      if (pz) put(a.gz, t0, oY);
+      const bool whole = L - tw >= TT;
+      put_all(co, whole, L - tw, q, on, oB);
+      Column<T> c = co;
+      c.row = co.row + ((T*)a.gdt - (T*)a.gu);
+      put_all(c, whole, L - tw, q, on, oG);
+      c.row = co.row + ((T*)a.gz - (T*)a.gu);
+      if (gate) put_all(c, whole, L - tw, q, on, oY);
+      co.move();
     }
   }
   __syncthreads();
-  float* red = &ex[0][0][0][0];
+  float* red = &ex[0][0][0];
   if constexpr (STATE) {
-    if (q == 0)
-#pragma unroll
-      for (int c = 0; c < CPL; ++c) red[w * CW + (lane >> 2) * CPL + c] = Ssum[c];
+    if (q == 0) red[w * 16 + (lane >> 2)] = Ssum;
     __syncthreads();
-    if (w == 0) {
+    if (w == 0 && on) {
       const int64_t r = ((int64_t)at.b * p.nseg + at.seg) * a.D + d;
-#pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (c < nch) {
-          float S = 0.0f;
-          for (int v = 0; v < kWaves; ++v) S += red[v * CW + (lane >> 2) * CPL + c];
-          if (q == 0) p.segs[r + c] = S;
-          mix_store<float, NPL>(p.segh + (r + c) * NP + q * NPL, ec[c]);
-        }
+      float S = 0.0f;
+      for (int v = 0; v < W; ++v) S += red[v * 16 + (lane >> 2)];
+      if (q == 0) p.segs[r] = S;
+      mix_store<float, NPL>(p.segh + r * NP + q * NPL, ec);
     }
   } else {
     // dA, dD, d(bias) of the workgroup: over the waves in order
-#pragma unroll
-    for (int c = 0; c < CPL; ++c) {
-      gD[c] = quad_sum(gD[c]);
-      gb[c] = quad_sum(gb[c]);
-      mix_store<float, NPL>(&ex[w][0][c][lane * NPL], gA[c]);
-      if (q < 2) ex[w][1][c][(lane >> 2) * 2 + q] = q ? gb[c] : gD[c];
-    }
+    gD = quad_sum(gD);
+    gb = quad_sum(gb);
+    mix_store<float, NPL>(&ex[w][0][lane * NPL], gA);
+    if (q < 2) ex[w][1][(lane >> 2) * 2 + q] = q ? gb : gD;
     __syncthreads();
-    if (w == 0) {
+    if (w == 0 && on) {
       const int64_t r = ((int64_t)at.b * p.nseg + at.seg) * a.D + d;
+      float s[NPL] = {}, x = 0.0f;
+      for (int v = 0; v < W; ++v) {
+        float y[NPL];
+        mix_load<float, NPL>(&ex[v][0][lane * NPL], y);
 #pragma unroll
-      for (int c = 0; c < CPL; ++c)
-        if (c < nch) {
-          float s[NPL] = {}, x = 0.0f;
-          for (int v = 0; v < kWaves; ++v) {
-            float y[NPL];
-            mix_load<float, NPL>(&ex[v][0][c][lane * NPL], y);
+        for (int j = 0; j < NPL; ++j) s[j] += y[j];
+        if (q < 2) x += ex[v][1][(lane >> 2) * 2 + q];
+      }
+      float* o = p.part_a + r * (N + 2);
 #pragma unroll
-            for (int j = 0; j < NPL; ++j) s[j] += y[j];
-            if (q < 2) x += ex[v][1][c][(lane >> 2) * 2 + q];
-          }
-          float* o = p.part_a + (r + c) * (N + 2);
+      for (int j = 0; j < NPL; ++j)
+        if (q * NPL + j < N) o[q * NPL + j] = s[j];
+      if (q < 2) o[N + q] = x;
+      if (a.gh0 && at.seg == 0)
 #pragma unroll
-          for (int j = 0; j < NPL; ++j)
-            if (q * NPL + j < N) o[q * NPL + j] = s[j];
-          if (q < 2) o[N + q] = x;
-          if (a.gh0 && at.seg == 0)
-#pragma unroll
-            for (int j = 0; j < NPL; ++j)
-              if (q * NPL + j < N) a.gh0[((int64_t)at.b * a.D + d + c) * N + q * NPL + j] = ec[c][j];
-        }
+        for (int j = 0; j < NPL; ++j)
+          if (q * NPL + j < N) a.gh0[((int64_t)at.b * a.D + d) * N + q * NPL + j] = ec[j];
     }
   }
 }
@@ -821,8 +797,8 @@ bool valid(const w2s_ssm_args* a) {
 }
 
 int npl_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-template <int NPL> constexpr int fwd_tile() { return kWaves * FwdShape<NPL>::TT; }
-template <int NPL> constexpr int bwd_tile() { return kWaves * BwdShape<NPL>::TT; }
+template <int NPL> constexpr int fwd_tile() { return FwdShape<NPL>::W * FwdShape<NPL>::TT; }
+template <int NPL> constexpr int bwd_tile() { return BwdShape<NPL>::W * BwdShape<NPL>::TT; }
 
 // Segments a sequence is cut into.  Cutting costs a second walk for the end states, so it pays only where the workgroups of whole sequences leave
 // most of the 256 CUs idle.
@@ -836,9 +812,9 @@ int segments(int64_t blocks, int ntile) {
 
 template <int NPL> Plan plan_of(const w2s_ssm_args* a, bool backward) {
   Plan p{};
-  const int cw = 16 * (backward ? BwdShape<NPL>::CPL : FwdShape<NPL>::CPL), tile = backward ? bwd_tile<NPL>() : fwd_tile<NPL>();
+  const int tile = backward ? bwd_tile<NPL>() : fwd_tile<NPL>();
   p.dg = a->D / a->G;
-  p.ncb = (p.dg + cw - 1) / cw;
+  p.ncb = (p.dg + 15) / 16;
   p.ntile = (int)(((int64_t)a->L + tile - 1) / tile);
   p.nseg = segments((int64_t)a->B * a->G * p.ncb, p.ntile);
   p.tps = (p.ntile + p.nseg - 1) / p.nseg;
@@ -847,9 +823,7 @@ template <int NPL> Plan plan_of(const w2s_ssm_args* a, bool backward) {
   p.nck = (int)(((int64_t)a->L + bwd_tile<NPL>() - 1) / bwd_tile<NPL>());
   const int e = esize(a->dtype);
   p.vbc = a->N % 4 == 0 && mix_aligned(a->Bm, a->sB_b, a->sB_l, 4, e) && a->sB_g % 4 == 0 && mix_aligned(a->Cm, a->sC_b, a->sC_l, 4, e) && a->sC_g % 4 == 0;
-  p.vch = p.dg % 2 == 0 && mix_aligned(a->u, a->su_b, a->su_l, 2, e) && mix_aligned(a->dt, a->sdt_b, a->sdt_l, 2, e) && mix_aligned(a->z, a->sz_b, a->sz_l, 2, e) &&
-          mix_aligned(a->gy, a->sg_b, a->sg_l, 2, e) && mix_aligned(a->y, 0, 0, 2, e) && mix_aligned(a->gu, 0, 0, 2, e) && mix_aligned(a->gdt, 0, 0, 2, e) &&
-          mix_aligned(a->gz, 0, 0, 2, e);
+  if (p.vbc && a->N == 4 * NPL) p.vbc = 2;
   return p;
 }
 
@@ -872,9 +846,9 @@ template <typename T, int NPL> int scan_fwd(const w2s_ssm_args* a, hipStream_t s
     if (!a->ws) return W2S_EINVAL;
     p.segh = (float*)a->ws;
     p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
-    ssm_fwd_kernel<T, NPL, true, false><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
+    ssm_fwd_kernel<T, NPL, true><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   }
-  ssm_fwd_kernel<T, NPL, false, false><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
+  ssm_fwd_kernel<T, NPL, false><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   W2S_CHECK_LAUNCH();
   return W2S_OK;
 }
@@ -889,14 +863,8 @@ template <typename T, int NPL> int scan_bwd(const w2s_ssm_args* a, hipStream_t s
   p.segh = p.part_a + a_floats(a, p);
   p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
   if (blocks) {
-    if (BwdShape<NPL>::CPL > 1 && p.vch) {
-      constexpr bool V = BwdShape<NPL>::CPL > 1;
-      if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true, V><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
-      ssm_bwd_kernel<T, NPL, false, V><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
-    } else {
-      if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true, false><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
-      ssm_bwd_kernel<T, NPL, false, false><<<(unsigned)blocks, kWaves * 64, 0, st>>>(*a, p);
-    }
+    if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    ssm_bwd_kernel<T, NPL, false><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   }
   if (nbc) ssm_reduce_bc_kernel<T><<<(unsigned)nbc, 256, 0, st>>>(*a, p.ncb, 4 * NPL, p.part_bc);
   ssm_reduce_a_kernel<<<(unsigned)na, 1024, 0, st>>>(*a, a->B * p.nseg, p.part_a);

@@ -99,8 +99,8 @@ READELF = os.path.join(os.path.dirname(OBJDUMP), 'llvm-readelf')
 SCRATCH_ALLOWED = {
     '_Z14conv_cl_kernelILi8ELi4ELi3ELi3ELi1ELi2E': 320, '_Z14conv_cl_kernelILi8ELi4ELi4ELi4ELi1ELi2E': 320, '_Z14conv_cl_kernelILi8ELi4ELi7ELi1ELi0ELi2E': 320,
     '_Z14conv_cl_kernelILi8ELi4ELi7ELi1ELi1ELi2E': 320, '_Z16bwd_fused_kernelILi1ELi1ELi4ELi0ELi1EE': 32, '_Z16conv_wide_kernelILi8ELi8ELi4ELi1ELi5ELi4ELi4ELi1ELi1E': 16,
-    # the scan's backward with 33 ... 64 states: 20 registers of loop invariants, outside the walks
-    '_ZN12_GLOBAL__N_114ssm_bwd_kernelIfLi16ELb0E': 80, '_ZN12_GLOBAL__N_114ssm_bwd_kernelIDF16bLi16ELb0E': 80, '_ZN12_GLOBAL__N_114ssm_bwd_kernelIDF16_Li16ELb0E': 80,
+    # the scan's backward with 33 ... 64 states: two to four registers of loop invariants, outside the walks
+    '_ZN12_GLOBAL__N_114ssm_bwd_kernelIfLi16ELb0E': 16, '_ZN12_GLOBAL__N_114ssm_bwd_kernelIDF16bLi16ELb0E': 16, '_ZN12_GLOBAL__N_114ssm_bwd_kernelIDF16_Li16ELb0E': 16,
 }
 
 
