@@ -45,22 +45,18 @@ template <typename T, int N> __device__ __forceinline__ void mix_store(T* p, con
 // 1 / (1 + e^-x); e^-x may overflow to inf (-> 0) and a NaN stays one
 __device__ __forceinline__ float mix_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
 
-// softplus(x) = max(x, 0) + log1p(e^-|x|).  With e = e^-|x| <= 1 and s = e / (2 + e) <= 1/3: log1p(e) = 2 atanh(s) = 2 (s + s^3/3 + s^5/5 + ...),
-// cut after s^15 / 15 (the next term is below 2^-30 of the sum): relative accuracy for tiny time steps too, where log(1 + e) has none
-__device__ __forceinline__ float mix_softplus(float x) {
+// softplus(x) = max(x, 0) + log1p(e) with e = e^-|x| <= 1, and its slope sigmoid(x) = (x > 0 ? 1 : e) / (1 + e).  log1p(e): w = 1 + e rounds e's low bits
+// away; c = e - (w - 1) is what was lost, exactly, and log(1 + e) = log(w) + c / w up to c^2.  For w in [1, 2] c / w and c differ by at most |c| e, half a
+// step of e, so the sum has full relative accuracy for tiny time steps too, where log(1 + e) alone has none.
+__device__ __forceinline__ float mix_softplus(float x, float& slope) {
   const float e = __builtin_amdgcn_exp2f(-1.4426950408889634f * __builtin_fabsf(x));
-  const float s = e * __builtin_amdgcn_rcpf(2.0f + e);
-  const float q = s * s;
-  float p = 1.0f / 15.0f;
-  p = __builtin_fmaf(p, q, 1.0f / 13.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 11.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 9.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 7.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 5.0f);
-  p = __builtin_fmaf(p, q, 1.0f / 3.0f);
-  p = __builtin_fmaf(p, q, 1.0f);
-  const float t = 2.0f * s * p;
-  return x > 0.0f ? x + t : (x == x ? t : x);
+  const float w = 1.0f + e, c = e - (w - 1.0f), r = __builtin_amdgcn_rcpf(w);
+  slope = x > 0.0f ? r : e * r;
+  return fmaxf(x, 0.0f) + __builtin_fmaf(__builtin_amdgcn_logf(w), 0.6931471805599453f, c);   // (a NaN comes through c)
+}
+__device__ __forceinline__ float mix_softplus(float x) {
+  float slope;
+  return mix_softplus(x, slope);
 }
 
 // sum over the lanes of an aligned group of G lanes (a power of two <= 64); every lane gets it, in one fixed order

@@ -70,8 +70,8 @@ __device__ __forceinline__ float sum_quads_of_row(float v) {   // over the four 
 #ifndef FW
 #define FW 16
 #define FT 8
-#define BW 16
-#define BT 4
+#define BW 8
+#define BT 8
 #endif
 template <int NPL> struct FwdShape { static constexpr int W = NPL <= 4 ? FW : 8, TT = NPL <= 4 ? FT : 64 / NPL; };
 template <int NPL> struct BwdShape { static constexpr int W = NPL <= 4 ? BW : 8, TT = NPL <= 4 ? BT : NPL <= 8 ? 8 : 4; };
@@ -104,18 +104,17 @@ __device__ __forceinline__ Where where_of(const w2s_ssm_args& a, const Plan& p) 
 // One channel's values of a tensor [L][channels], four positions to a quad (lane q has positions 4 i + q of its wave's TT): a wave-uniform running row, moved
 // on a tile at a time, and one 32-bit lane offset, so that an access is a scalar base and an offset and costs no 64-bit arithmetic a lane.
 template <typename T> struct Column {
-  T* row;           // position 0 of this wave's TT in the current tile, the group's first channel
-  int64_t four, tile;
+  T* row;         // position 0 of this wave's TT in the current tile, the group's first channel
+  int sl;         // elements from position to position (below 2^22)
   unsigned off;
-  __device__ __forceinline__ void start(const void* base, int64_t sb, int64_t sl, int b, int channel0, int t, int tile_step, int q, int ch) {
-    row = (T*)base + b * sb + t * sl + channel0;
-    four = 4 * sl;
-    tile = tile_step * sl;
+  __device__ __forceinline__ void start(const void* base, int64_t sb, int64_t stride, int b, int channel0, int t, int q, int ch) {
+    sl = (int)stride;
+    row = (T*)base + b * sb + t * stride + channel0;
     off = (unsigned)(q * sl) + ch;
   }
-  __device__ __forceinline__ void move() { row += tile; }
-  __device__ __forceinline__ T get(int i) const { return (row + i * four)[(unsigned)forgotten(off)]; }
-  __device__ __forceinline__ void put(int i, float v) const { (row + i * four)[(unsigned)forgotten(off)] = (T)v; }
+  template <int TILE> __device__ __forceinline__ void move() { row += TILE * sl; }
+  __device__ __forceinline__ T get(int i) const { return (row + i * 4 * sl)[(unsigned)forgotten(off)]; }
+  __device__ __forceinline__ void put(int i, float v) const { (row + i * 4 * sl)[(unsigned)forgotten(off)] = (T)v; }
 };
 // (values stay in the memory's type until a tile is worked on: a conversion here would wait for the load that it is to hide)
 template <typename T, int NI> __device__ __forceinline__ void get_all(const Column<const T>& c, bool whole, int left, int q, T (&v)[NI]) {   // left: positions up to L
@@ -146,24 +145,24 @@ template <typename T, int NP, int TILE, int W> struct StageBC {
   static constexpr int HALF = TILE * NP / 4, PER = (2 * HALF + W * 64 - 1) / (W * 64);
   static_assert(HALF % 64 == 0, "a wave's units are all of B or all of C");
   const T *rowB, *rowC;   // the tile's first position
-  int64_t tileB, tileC;
+  int slB, slC;
   unsigned off[PER];
   typedef typename mix_vec<T, 4>::type V;
   V v[PER];
-  __device__ __forceinline__ void start(const w2s_ssm_args& a, const Where& at, int t, int tile_step, int w, int lane) {
+  __device__ __forceinline__ void start(const w2s_ssm_args& a, const Where& at, int t, int w, int lane) {
     rowB = (const T*)a.Bm + at.b * a.sB_b + at.g * a.sB_g + t * a.sB_l;
     rowC = (const T*)a.Cm + at.b * a.sC_b + at.g * a.sC_g + t * a.sC_l;
-    tileB = tile_step * a.sB_l;
-    tileC = tile_step * a.sC_l;
+    slB = (int)a.sB_l;
+    slC = (int)a.sC_l;
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int u0 = (k * W + w) * 64, isc = u0 >= HALF, r = u0 - isc * HALF + lane;
-      off[k] = r / (NP / 4) * (unsigned)(isc ? a.sC_l : a.sB_l) + r % (NP / 4) * 4;
+      off[k] = r / (NP / 4) * (isc ? slC : slB) + r % (NP / 4) * 4;
     }
   }
-  __device__ __forceinline__ void move() {
-    rowB += tileB;
-    rowC += tileC;
+  template <int STEP> __device__ __forceinline__ void move() {
+    rowB += STEP * slB;
+    rowC += STEP * slC;
   }
   __device__ __forceinline__ void load(const w2s_ssm_args& a, int vbc, int left, bool with_c, int w, int lane) {   // left: positions of the tile up to L
 #pragma unroll
@@ -200,8 +199,8 @@ template <typename T, int NP, int TILE, int W> struct StageBC {
 };
 
 // ------------------------------------------------------------------------------------------------------------------ forward
-// STATE: only the segment's end state (from zero) and its sum of delta
-template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape<NPL>::W * 64) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
+// GATE: z is there.  STATE: only the segment's end state (from zero) and its sum of delta
+template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds__(FwdShape<NPL>::W * 64) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
   constexpr int W = FwdShape<NPL>::W, TT = FwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL;
   constexpr int CK = BwdShape<NPL>::W * BwdShape<NPL>::TT;   // positions between the states that the backward starts from
   __shared__ float bc[2][TILE * NP * 2];
@@ -213,7 +212,6 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
   const int ch = on ? at.cb * 16 + (lane >> 2) : p.dg - 1, dg0 = at.g * p.dg, d = dg0 + ch;
   const int n = mix_length(a.lengths, at.b, a.L), N = a.N, L = a.L;
   const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
-  const bool gate = !STATE && a.z;
   float A[NPL], hc[NPL];
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
@@ -235,12 +233,12 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
   const int t00 = k0 * TILE + w * TT;
   Column<const T> cu, cd, cz;
   Column<T> cy;
-  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, TILE, q, ch);
-  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, TILE, q, ch);
-  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, TILE, q, ch);
-  cy.start(a.y, (int64_t)L * a.D, a.D, at.b, dg0, t00, TILE, q, ch);
+  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, q, ch);
+  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, q, ch);
+  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, q, ch);
+  cy.start(a.y, (int64_t)L * a.D, a.D, at.b, dg0, t00, q, ch);
   StageBC<T, NP, TILE, W> st;
-  st.start(a, at, k0 * TILE, TILE, w, lane);
+  st.start(a, at, k0 * TILE, w, lane);
   T ru[NI], rd[NI], rz[NI];
   float Ssum = 0.0f;
   auto fetch = [&](int t0) {   // ... and on to the tile behind it
@@ -248,12 +246,12 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
     const bool whole = left >= TT;
     get_all(cu, whole, left, q, ru);
     get_all(cd, whole, left, q, rd);
-    if (gate) get_all(cz, whole, left, q, rz);
+    if (GATE) get_all(cz, whole, left, q, rz);
     st.load(a, p.vbc, L - t0, !STATE, w, lane);
-    cu.move();
-    cd.move();
-    cz.move();
-    st.move();
+    cu.template move<TILE>();
+    cd.template move<TILE>();
+    cz.template move<TILE>();
+    st.template move<TILE>();
   };
   if (k0 < k1 && k0 * TILE < n) fetch(k0 * TILE);
   for (int k = k0; k < k1; ++k) {
@@ -262,7 +260,7 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
       if (!STATE) {
         const float zero[NI] = {};
         put_all(cy, L - tw >= TT, L - tw, q, on, zero);
-        cy.move();
+        cy.template move<TILE>();
       }
       continue;
     }
@@ -349,7 +347,7 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) y[i] = __builtin_fmaf(Dp, u[i], y[i]);
-      if (gate) {
+      if (GATE) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) y[i] *= z[i] * mix_sigmoid(z[i]);
       }
@@ -358,7 +356,7 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
         for (int i = 0; i < NI; ++i) y[i] = 4 * i + q < n - tw ? y[i] : 0.0f;
       }
       put_all(cy, L - tw >= TT, L - tw, q, on, y);
-      cy.move();
+      cy.template move<TILE>();
     }
   }
   if constexpr (STATE) {
@@ -386,7 +384,7 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(FwdShape
 // for h, backward for e), meet in LDS, and walk both ways again from the right ends, the states of the second walk staying in registers.  dB and dC are
 // summed over the 16 channels of a workgroup by lane exchanges and over workgroups from `part_bc`; everything in a fixed order.
 // STATE: only e at the segment's start (from zero) and the sum of delta.
-template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape<NPL>::W * 64) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
+template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds__(BwdShape<NPL>::W * 64) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
   constexpr int W = BwdShape<NPL>::W, TT = BwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL, NX = STATE ? 2 : 3;
   __shared__ float bc[2][TILE * NP * 2];
   __shared__ float ex[W][NX][64 * NPL];
@@ -397,7 +395,7 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
   const int ch = on ? at.cb * 16 + (lane >> 2) : p.dg - 1, dg0 = at.g * p.dg, d = dg0 + ch;
   const int n = mix_length(a.lengths, at.b, a.L), N = a.N, L = a.L;
   const int k0 = at.seg * p.tps, k1 = k0 + p.tps < p.ntile ? k0 + p.tps : p.ntile;
-  const bool gate = a.z != nullptr, has_gy = a.gy != nullptr;
+  const bool has_gy = a.gy != nullptr;
   float A[NPL], ec[NPL], gA[NPL], gD = 0.0f, gb = 0.0f, Ssum = 0.0f;
 #pragma unroll
   for (int j = 0; j < NPL; ++j) {
@@ -425,37 +423,37 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
       const int tw = k * TILE + w * TT;
       const float zero[NI] = {};
       Column<T> c;
-      c.start(a.gu, LD, a.D, at.b, dg0, tw, 0, q, ch);
+      c.start(a.gu, LD, a.D, at.b, dg0, tw, q, ch);
       put_all(c, false, L - tw, q, on, zero);
-      c.start(a.gdt, LD, a.D, at.b, dg0, tw, 0, q, ch);
+      c.start(a.gdt, LD, a.D, at.b, dg0, tw, q, ch);
       put_all(c, false, L - tw, q, on, zero);
-      c.start(a.gz, LD, a.D, at.b, dg0, tw, 0, q, ch);
-      if (gate) put_all(c, false, L - tw, q, on, zero);
+      c.start(a.gz, LD, a.D, at.b, dg0, tw, q, ch);
+      if (GATE) put_all(c, false, L - tw, q, on, zero);
     }
   const int t00 = (kl - 1) * TILE + w * TT;
   Column<const T> cu, cd, cz, cg;
   Column<T> co;   // one row pointer for the three outputs, which are alike: gdt and gz at fixed distances
-  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, -TILE, q, ch);
-  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, -TILE, q, ch);
-  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, -TILE, q, ch);
-  cg.start(a.gy, a.sg_b, a.sg_l, at.b, dg0, t00, -TILE, q, ch);
-  co.start(a.gu, LD, a.D, at.b, dg0, t00, -TILE, q, ch);
+  cu.start(a.u, a.su_b, a.su_l, at.b, dg0, t00, q, ch);
+  cd.start(a.dt, a.sdt_b, a.sdt_l, at.b, dg0, t00, q, ch);
+  cz.start(a.z, a.sz_b, a.sz_l, at.b, dg0, t00, q, ch);
+  cg.start(a.gy, a.sg_b, a.sg_l, at.b, dg0, t00, q, ch);
+  co.start(a.gu, LD, a.D, at.b, dg0, t00, q, ch);
   StageBC<T, NP, TILE, W> st;
-  st.start(a, at, (kl - 1) * TILE, -TILE, w, lane);
+  st.start(a, at, (kl - 1) * TILE, w, lane);
   T ru[NI], rd[NI], rz[NI], rg[NI];
   auto fetch = [&](int t0) {   // ... and on to the tile in front of it
     const int left = L - t0 - w * TT;
     const bool whole = left >= TT;
     if (!STATE) get_all(cu, whole, left, q, ru);
     get_all(cd, whole, left, q, rd);
-    if (gate) get_all(cz, whole, left, q, rz);
+    if (GATE) get_all(cz, whole, left, q, rz);
     if (has_gy) get_all(cg, whole, left, q, rg);
     st.load(a, p.vbc, L - t0, true, w, lane);
-    cu.move();
-    cd.move();
-    cz.move();
-    cg.move();
-    st.move();
+    cu.template move<-TILE>();
+    cd.template move<-TILE>();
+    cz.template move<-TILE>();
+    cg.template move<-TILE>();
+    st.template move<-TILE>();
   };
   // where a lane leaves its share of dB and dC (the walk's reduction below)
   const unsigned out_off = NPL < 4 ? ((lane >> 4) & 1) * NP + q * NPL + (lane >> 5) : (lane & 4 ? NP : 0) + q * NPL + ((lane >> 4) & 1) * 2 + (lane >> 5);
@@ -463,12 +461,13 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
   if (kl > k0) fetch((kl - 1) * TILE);
   for (int k = kl - 1; k >= k0; --k) {
     const int t0 = k * TILE, par = (kl - 1 - k) & 1, tw = t0 + w * TT;
-    float u[NI], dl[NI], du[NI], raw[NI], gp[NI], gy[NI], z[NI], S = 0.0f, hi[NPL];
+    float u[NI], dl[NI], du[NI], slope[NI], gp[NI], gy[NI], z[NI], sz[NI], S = 0.0f, hi[NPL];
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      raw[i] = (float)rd[i] + bias;
+      const float r = (float)rd[i] + bias;
       u[i] = STATE ? 0.0f : (float)ru[i];
-      dl[i] = a.softplus ? mix_softplus(raw[i]) : raw[i];
+      slope[i] = 1.0f;
+      dl[i] = a.softplus ? mix_softplus(r, slope[i]) : r;
       gy[i] = has_gy ? (float)rg[i] : 0.0f;
       z[i] = (float)rz[i];
     }
@@ -480,13 +479,14 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
         dl[i] = live ? dl[i] : 0.0f;
         gy[i] = live ? gy[i] : 0.0f;
         z[i] = live ? z[i] : 0.0f;
-        raw[i] = live ? raw[i] : 0.0f;
+        slope[i] = live ? slope[i] : 0.0f;
       }
     }
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       du[i] = dl[i] * u[i];
-      gp[i] = gate ? gy[i] * z[i] * mix_sigmoid(z[i]) : gy[i];
+      sz[i] = GATE ? mix_sigmoid(z[i]) : 0.0f;
+      gp[i] = GATE ? gy[i] * z[i] * sz[i] : gy[i];
       S += dl[i];
     }
     float* lds = bc[par];
@@ -563,7 +563,8 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
       // The second walk in parts of HALF positions from the last part to the first, so that only a part's states are in registers; h first reaches a
       // part's start without keeping any.
       constexpr int HALF = NPL <= 4 ? TT : NPL == 8 ? 2 : 1, PARTS = TT / HALF, JB = NPL < 4 ? NPL : 4;
-      float oB[NI], oG[NI], oY[NI];
+      constexpr bool LATE = NPL <= 4;   // a lane's shares of dB and dC wait in registers for the walk's end, which then has no branch inside
+      float oB[NI], oG[NI], oY[NI], share[TT];
       forget(gp);
       if (!KEEP) forget(A);
       auto forward = [&](const float* x, int t, float* to) {
@@ -626,30 +627,36 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
             } else {
               v = sum_quads_of_row(fold16(fold32(pb[0], pb[1]), fold32(pc[0], pc[1])));
             }
-            if (out_on && t < n - tw) (row + j0)[(unsigned)forgotten(out_off)] = v;
+            if (LATE) share[t] = v;
+            else if (out_on && t < n - tw) (row + j0)[(unsigned)forgotten(out_off)] = v;
           }
           const bool mine = q == (t & 3) || (t & 3) == 3;   // (the highest of a lane's four comes first; the others then choose)
-          const float vB = quad_sum(sB), vG = quad_sum(sG), vY = gate ? quad_sum(sY) : 0.0f;
+          const float vB = quad_sum(sB), vG = quad_sum(sG), vY = GATE ? quad_sum(sY) : 0.0f;
           oB[t / 4] = mine ? vB : oB[t / 4];
           oG[t / 4] = mine ? vG : oG[t / 4];
           oY[t / 4] = mine ? vY : oY[t / 4];
-          __builtin_amdgcn_sched_barrier(0);
+          if (!LATE) __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (LATE && out_on) {
+        const int step = a.G * 2 * NP;
+        if (n - tw >= TT) {
+#pragma unroll
+          for (int t = 0; t < TT; ++t) (out + t * step)[(unsigned)forgotten(out_off)] = share[t];
+        } else {
+#pragma unroll
+          for (int t = 0; t < TT; ++t)
+            if (t < n - tw) (out + t * step)[(unsigned)forgotten(out_off)] = share[t];
         }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {   // (behind the end u, delta, gy, z and G are zero, and so is all of this but the sigmoid's factor)
-        float gd = __builtin_fmaf(kLn2, oG[i], u[i] * oB[i]);
-        if (a.softplus) gd *= mix_sigmoid(raw[i]);
-        const bool live = 4 * i + q < n - tw;
-        oG[i] = live ? gd : 0.0f;
-        const float gu = live ? __builtin_fmaf(dl[i], oB[i], Dp * gp[i]) : 0.0f;
+      for (int i = 0; i < NI; ++i) {   // (behind the end u, delta, its slope, gy and gy' are zero, and so are these)
+        const float gd = slope[i] * __builtin_fmaf(kLn2, oG[i], u[i] * oB[i]);
+        oB[i] = __builtin_fmaf(dl[i], oB[i], Dp * gp[i]);
         gD = __builtin_fmaf(gp[i], u[i], gD);
-        gb += oG[i];
-        if (gate) {
-          const float s = mix_sigmoid(z[i]);
-          oY[i] = gy[i] * __builtin_fmaf(Dp, u[i], oY[i]) * s * (1.0f + z[i] * (1.0f - s));
-        }
-        oB[i] = gu;
+        gb += gd;
+        oG[i] = gd;
+        if (GATE) oY[i] = gy[i] * __builtin_fmaf(Dp, u[i], oY[i]) * sz[i] * (1.0f + z[i] * (1.0f - sz[i]));
       }
       const bool whole = L - tw >= TT;
       put_all(co, whole, L - tw, q, on, oB);
@@ -657,8 +664,8 @@ template <typename T, int NPL, bool STATE> __global__ __launch_bounds__(BwdShape
       c.row = co.row + ((T*)a.gdt - (T*)a.gu);
       put_all(c, whole, L - tw, q, on, oG);
       c.row = co.row + ((T*)a.gz - (T*)a.gu);
-      if (gate) put_all(c, whole, L - tw, q, on, oY);
-      co.move();
+      if (GATE) put_all(c, whole, L - tw, q, on, oY);
+      co.template move<-TILE>();
     }
   }
   __syncthreads();
@@ -838,7 +845,7 @@ template <int NPL> int64_t ws_floats(const w2s_ssm_args* a, bool backward) {
 
 template <int NPL> int64_t ckpt_floats(const w2s_ssm_args* a) { return (int64_t)a->B * plan_of<NPL>(a, false).nck * a->D * 4 * NPL; }
 
-template <typename T, int NPL> int scan_fwd(const w2s_ssm_args* a, hipStream_t st) {
+template <typename T, int NPL, bool GATE> int scan_fwd(const w2s_ssm_args* a, hipStream_t st) {
   Plan p = plan_of<NPL>(a, false);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
   if (blocks > 0x7fffffff) return W2S_EINVAL;
@@ -846,14 +853,14 @@ template <typename T, int NPL> int scan_fwd(const w2s_ssm_args* a, hipStream_t s
     if (!a->ws) return W2S_EINVAL;
     p.segh = (float*)a->ws;
     p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
-    ssm_fwd_kernel<T, NPL, true><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    ssm_fwd_kernel<T, NPL, true, false><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   }
-  ssm_fwd_kernel<T, NPL, false><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+  ssm_fwd_kernel<T, NPL, false, GATE><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   W2S_CHECK_LAUNCH();
   return W2S_OK;
 }
 
-template <typename T, int NPL> int scan_bwd(const w2s_ssm_args* a, hipStream_t st) {
+template <typename T, int NPL, bool GATE> int scan_bwd(const w2s_ssm_args* a, hipStream_t st) {
   Plan p = plan_of<NPL>(a, true);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
   const int64_t rows = (int64_t)a->B * a->L * a->G, nbc = (rows * (2 * NPL) + 255) / 256, na = ((int64_t)a->D * (a->N + 2) + 63) / 64;
@@ -863,8 +870,8 @@ template <typename T, int NPL> int scan_bwd(const w2s_ssm_args* a, hipStream_t s
   p.segh = p.part_a + a_floats(a, p);
   p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
   if (blocks) {
-    if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
-    ssm_bwd_kernel<T, NPL, false><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true, GATE><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    ssm_bwd_kernel<T, NPL, false, GATE><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
   }
   if (nbc) ssm_reduce_bc_kernel<T><<<(unsigned)nbc, 256, 0, st>>>(*a, p.ncb, 4 * NPL, p.part_bc);
   ssm_reduce_a_kernel<<<(unsigned)na, 1024, 0, st>>>(*a, a->B * p.nseg, p.part_a);
@@ -872,12 +879,17 @@ template <typename T, int NPL> int scan_bwd(const w2s_ssm_args* a, hipStream_t s
   return W2S_OK;
 }
 
+template <typename T, int NPL> int by_gate(const w2s_ssm_args* a, bool backward, hipStream_t st) {
+  if (a->z) return backward ? scan_bwd<T, NPL, true>(a, st) : scan_fwd<T, NPL, true>(a, st);
+  return backward ? scan_bwd<T, NPL, false>(a, st) : scan_fwd<T, NPL, false>(a, st);
+}
+
 template <typename T> int by_states(const w2s_ssm_args* a, bool backward, hipStream_t st) {
   switch (npl_of(a->N)) {
-    case 2: return backward ? scan_bwd<T, 2>(a, st) : scan_fwd<T, 2>(a, st);
-    case 4: return backward ? scan_bwd<T, 4>(a, st) : scan_fwd<T, 4>(a, st);
-    case 8: return backward ? scan_bwd<T, 8>(a, st) : scan_fwd<T, 8>(a, st);
-    default: return backward ? scan_bwd<T, 16>(a, st) : scan_fwd<T, 16>(a, st);
+    case 2: return by_gate<T, 2>(a, backward, st);
+    case 4: return by_gate<T, 4>(a, backward, st);
+    case 8: return by_gate<T, 8>(a, backward, st);
+    default: return by_gate<T, 16>(a, backward, st);
   }
 }
 
