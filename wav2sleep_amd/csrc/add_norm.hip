@@ -276,17 +276,10 @@ template <typename T, typename RT> __global__ __launch_bounds__(256) void add_no
 }
 
 __global__ __launch_bounds__(1024) void add_norm_reduce_kernel(const float* part, int nparts, int C, float* gw) {
-  __shared__ float red[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), row = threadIdx.x >> 6;
-  float v = 0.0f;
-  if (col < C)
-    for (int p = row; p < nparts; p += 16) v += part[(int64_t)p * C + col];
-  red[row][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (row == 0 && col < C) {
-    for (int q = 1; q < 16; ++q) v += red[q][threadIdx.x];
-    gw[col] = v;
-  }
+  __shared__ float red[64][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15);
+  const float v = mix_part_sum(part, nparts, C, col, red);
+  if (threadIdx.x < 16 && col < C) gw[col] = v;
 }
 
 int esize(int dtype) { return dtype == W2S_F32 ? 4 : 2; }
@@ -353,7 +346,7 @@ int dispatch(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
     case W2S_BF16: wide_r ? by_width<bf16_t, float>(a, bwd, st) : by_width<bf16_t, bf16_t>(a, bwd, st); break;
     case W2S_F16: wide_r ? by_width<half_t, float>(a, bwd, st) : by_width<half_t, half_t>(a, bwd, st); break;
   }
-  if (bwd && a->gw) add_norm_reduce_kernel<<<(a->C + 63) / 64, 1024, 0, st>>>(a->part, bwd_blocks(a), a->C, a->gw);
+  if (bwd && a->gw) add_norm_reduce_kernel<<<(a->C + 15) / 16, 1024, 0, st>>>(a->part, bwd_blocks(a), a->C, a->gw);
   W2S_CHECK_LAUNCH();
   return W2S_OK;
 }

@@ -77,6 +77,24 @@ __device__ __forceinline__ int mix_length(const int32_t* lengths, int b, int L) 
   return n < 0 ? 0 : (n > L ? L : n);
 }
 
+// sum over `nparts` rows of part[row][C] at column col of the workgroup's 16 (1024 threads = 64 strided row sums x 16 columns, then a tree: a fixed order);
+// valid in the 16 threads of row 0
+__device__ __forceinline__ float mix_part_sum(const float* part, int nparts, int64_t C, int64_t col, float (*red)[17]) {
+  const int c = threadIdx.x & 15, r = threadIdx.x >> 4;
+  float v = 0.0f;
+  if (col < C) {
+#pragma unroll 4
+    for (int p = r; p < nparts; p += 64) v += part[(int64_t)p * C + col];
+  }
+  red[r][c] = v;
+#pragma unroll
+  for (int h = 32; h; h >>= 1) {
+    __syncthreads();
+    if (r < h) red[r][c] = v += red[r + h][c];
+  }
+  return v;
+}
+
 static inline bool mix_aligned(const void* p, int64_t s0, int64_t s1, int vec, int esize) {   // base and both strides allow vec-element accesses
   return ((uintptr_t)p % (size_t)(vec * esize)) == 0 && s0 % vec == 0 && s1 % vec == 0;
 }

@@ -8,7 +8,7 @@ namespace {
 
 constexpr int kRun = 8;   // positions per thread: 8 + K - 1 loads of 16 bytes in flight per lane
 
-struct Shape { int ncg, cx, ty, ncgb, nchb, L, D; };
+struct Shape { int ncg, cx, ty, ncgb, nchb, L, D, runs; };   // runs: how many runs of positions a thread of the backward takes, ty runs apart
 
 // rows r of [state; x] as floats; r counts from the first state row, n = length
 template <typename T, int VEC, int K>
@@ -90,16 +90,16 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   blk /= s.ncgb;
   const int chb = blk % s.nchb, b = blk / s.nchb;
   const int cx = (int)threadIdx.x % s.cx, ty = (int)threadIdx.x / s.cx;
-  const int cg = cgb * s.cx + cx, ch = chb * s.ty + ty;
-  const int t0 = ch * kRun, D = s.D;
-  const bool on = cg < s.ncg && (t0 < s.L || ch == 0);
-  const int d = on ? cg * VEC : 0, n = mix_length(a.lengths, b, s.L);
+  const int cg = cgb * s.cx + cx, D = s.D;
+  const int d = cg < s.ncg ? cg * VEC : 0, n = mix_length(a.lengths, b, s.L);
   float gwk[K + 1][VEC];
 #pragma unroll
   for (int k = 0; k <= K; ++k)
 #pragma unroll
     for (int c = 0; c < VEC; ++c) gwk[k][c] = 0.0f;
-  if (on) {
+  for (int run = 0; run < s.runs; ++run) {
+    const int ch = (chb * s.runs + run) * s.ty + ty, t0 = ch * kRun;
+    if (cg >= s.ncg || (t0 >= s.L && ch > 0)) break;
     const T* x = (const T*)a.x + b * a.sx_b + d;
     const T* g = a.gy ? (const T*)a.gy + b * a.sg_b + d : nullptr;
     const T* state = a.state ? (const T*)a.state + (int64_t)b * (K - 1) * D + d : nullptr;
@@ -213,18 +213,13 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   }
 }
 
-// gw[d][k] / gbias[d] = sum over workgroups of part[p][k][d]: 64 columns x 16 strided row sums per workgroup, then those 16 in order
+// gw[d][k] / gbias[d] = sum over workgroups of part[p][k][d]
 __global__ __launch_bounds__(1024) void short_conv_reduce_kernel(const float* part, int nparts, int K, int D, float* gw, float* gbias) {
-  __shared__ float red[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), row = threadIdx.x >> 6, C = (K + 1) * D;
-  float v = 0.0f;
-  if (col < C)
-    for (int p = row; p < nparts; p += 16) v += part[(int64_t)p * C + col];
-  red[row][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (row == 0 && col < C) {
-    for (int q = 1; q < 16; ++q) v += red[q][threadIdx.x];
-    const int k = col / D, d = col % D;
+  __shared__ float red[64][17];
+  const int64_t C = (int64_t)(K + 1) * D, col = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  const float v = mix_part_sum(part, nparts, C, col, red);
+  if (threadIdx.x < 16 && col < C) {
+    const int k = (int)(col / D), d = (int)(col % D);
     if (k < K) {
       if (gw) gw[(int64_t)d * K + k] = v;
     } else if (gbias) {
@@ -255,7 +250,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   for (int k = 0; k < K - 1; ++k) mix_store<T, VEC>((T*)a.state_out + ((int64_t)b * (K - 1) + k) * D + d, win[k + 1]);   // all loads are done: in place is fine
 }
 
-Shape shape_of(const w2s_short_conv_args* a, int vec) {
+Shape shape_of(const w2s_short_conv_args* a, int vec, bool backward) {
   Shape s;
   s.L = a->L;
   s.D = a->D;
@@ -266,6 +261,12 @@ Shape shape_of(const w2s_short_conv_args* a, int vec) {
   s.ncgb = (s.ncg + s.cx - 1) / s.cx;
   const int nch = a->L > 0 ? (a->L + kRun - 1) / kRun : 1;   // (an empty sequence still hands its state on)
   s.nchb = (nch + s.ty - 1) / s.ty;
+  s.runs = 1;
+  // the sums that a workgroup of the backward leaves are K + 1 floats a channel: with more workgroups than fill the chip (8 a CU) it takes several runs
+  while (backward && (int64_t)a->B * s.nchb * s.ncgb > 2048 && s.nchb > 1 && s.runs < 16) {
+    s.runs *= 2;
+    s.nchb = (s.nchb + 1) / 2;
+  }
   return s;
 }
 
@@ -291,13 +292,13 @@ enum { kFwd, kBwd, kStep };
 
 template <typename T, int VEC, int K, bool BWD> int launch(const w2s_short_conv_args* a, int what, hipStream_t st) {
   if constexpr (BWD) {
-    const Shape s = shape_of(a, VEC);
+    const Shape s = shape_of(a, VEC, true);
     const int64_t blocks = (int64_t)a->B * s.nchb * s.ncgb;
     if (blocks > 0x7fffffff) return W2S_EINVAL;
     short_conv_bwd_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, s);
     if (a->part) {
       const int64_t C = (int64_t)(K + 1) * a->D;
-      short_conv_reduce_kernel<<<(unsigned)((C + 63) / 64), 1024, 0, st>>>(a->part, a->B * s.nchb, K, a->D, a->gw, a->gbias);
+      short_conv_reduce_kernel<<<(unsigned)((C + 15) / 16), 1024, 0, st>>>(a->part, a->B * s.nchb, K, a->D, a->gw, a->gbias);
     }
   } else if (what == kStep) {
     const int ncg = a->D / VEC;
@@ -305,7 +306,7 @@ template <typename T, int VEC, int K, bool BWD> int launch(const w2s_short_conv_
     if (blocks > 0x7fffffff) return W2S_EINVAL;
     short_conv_step_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, ncg);
   } else {
-    const Shape s = shape_of(a, VEC);
+    const Shape s = shape_of(a, VEC, false);
     const int64_t blocks = (int64_t)a->B * s.nchb * s.ncgb;
     if (blocks > 0x7fffffff) return W2S_EINVAL;
     short_conv_fwd_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, s);
@@ -355,7 +356,7 @@ extern "C" int w2s_short_conv_fwd(const w2s_short_conv_args* a, void* stream) {
 
 extern "C" int64_t w2s_short_conv_part(const w2s_short_conv_args* a) {
   if (!valid(a)) return W2S_EINVAL;
-  const Shape s = shape_of(a, vector_of(a, true));
+  const Shape s = shape_of(a, vector_of(a, true), true);
   return (int64_t)a->B * s.nchb * (a->K + 1) * a->D;
 }
 

@@ -65,19 +65,15 @@ __device__ __forceinline__ float sum_quads_of_row(float v) {   // over the four 
   return v;
 }
 
-// tile shapes by states per lane: W waves, TT positions a wave.  Sixteen waves of few positions hide each other's LDS and barrier waits (four a SIMD, which
-// 128 registers a lane allow); from eight states a lane on the registers of a walk leave two a SIMD.
-#ifndef FW
-#define FW 16
-#define FT 8
-#define BW 8
-#define BT 8
-#endif
-template <int NPL> struct FwdShape { static constexpr int W = NPL <= 4 ? FW : 8, TT = NPL <= 4 ? FT : 64 / NPL; };
-template <int NPL> struct BwdShape { static constexpr int W = NPL <= 4 ? BW : 8, TT = NPL <= 4 ? BT : NPL <= 8 ? 8 : 4; };
+// Tile shapes: W waves, TT positions a wave, SIMD waves a SIMD (what the registers have to allow).  WIDE where there is at most one workgroup a CU (and nothing to be gained from cutting sequences): the forward then
+// takes sixteen waves, which hide each other's LDS and barrier waits, and the backward eight with a long walk each.  With more workgroups than CUs, eight
+// waves of at most 128 registers a lane, so that a CU holds two workgroups and the last round of them is short.  From eight states a lane on the registers
+// of a walk leave one.
+template <int NPL, bool WIDE> struct FwdShape { static constexpr int W = NPL <= 4 && WIDE ? 16 : 8, TT = NPL <= 8 ? 8 : 4, SIMD = NPL <= 4 ? 4 : 2; };
+template <int NPL, bool WIDE> struct BwdShape { static constexpr int W = 8, TT = NPL == 16 || (NPL <= 4 && !WIDE) ? 4 : 8, SIMD = NPL <= 4 && !WIDE ? 4 : 2; };
 
 struct Plan {
-  int dg, ncb, ntile, nseg, tps, nck, vbc;   // channels a group, channel blocks a group, tiles, segments, tiles a segment, checkpoints a sequence; B / C: 0 one by one, 1 by fours, 2 and N needs no padding
+  int dg, ncb, ntile, nseg, tps, ck, nck, vbc;   // channels a group, channel blocks a group, tiles, segments, tiles a segment, positions from checkpoint to checkpoint (the backward's tile) and how many; B / C: 0 one by one, 1 by fours, 2 and N needs no padding
   float *segh, *segs;                        // [B][nseg][D][NP] end states, [B][nseg][D] sums of delta (nseg > 1)
   float *part_bc, *part_a;                   // backward: [channel block][B][L][G][2 NP], [B nseg][D][N + 2]
 };
@@ -200,9 +196,8 @@ template <typename T, int NP, int TILE, int W> struct StageBC {
 
 // ------------------------------------------------------------------------------------------------------------------ forward
 // GATE: z is there.  STATE: only the segment's end state (from zero) and its sum of delta
-template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds__(FwdShape<NPL>::W * 64) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
-  constexpr int W = FwdShape<NPL>::W, TT = FwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL;
-  constexpr int CK = BwdShape<NPL>::W * BwdShape<NPL>::TT;   // positions between the states that the backward starts from
+template <typename T, int NPL, bool STATE, bool GATE, bool WIDE> __global__ __launch_bounds__((FwdShape<NPL, WIDE>::W * 64), (FwdShape<NPL, WIDE>::SIMD)) void ssm_fwd_kernel(w2s_ssm_args a, Plan p) {
+  constexpr int W = FwdShape<NPL, WIDE>::W, TT = FwdShape<NPL, WIDE>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL;
   __shared__ float bc[2][TILE * NP * 2];
   __shared__ float ex[W][2][64 * NPL];
   __shared__ float carry[2][64 * NPL];   // the state in front of a tile, from the last wave of the tile before
@@ -328,8 +323,8 @@ template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds
       mix_store<float, NPL>(&carry[par ^ 1][lane * NPL], hc);
     }
     if constexpr (!STATE) {
-      if (a.ckpt && (w * TT) % CK == 0 && tw < n && on)
-        mix_store<float, NPL>(a.ckpt + (((int64_t)at.b * p.nck + tw / CK) * a.D + dg0) * NP + (unsigned)(ch * NP + q * NPL), h);
+      if (a.ckpt && ((w * TT) & (p.ck - 1)) == 0 && tw < n && on)   // (a power of two, at most a tile)
+        mix_store<float, NPL>(a.ckpt + (((int64_t)at.b * p.nck + tw / p.ck) * a.D + dg0) * NP + (unsigned)(ch * NP + q * NPL), h);
       float y[NI];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -384,8 +379,8 @@ template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds
 // for h, backward for e), meet in LDS, and walk both ways again from the right ends, the states of the second walk staying in registers.  dB and dC are
 // summed over the 16 channels of a workgroup by lane exchanges and over workgroups from `part_bc`; everything in a fixed order.
 // STATE: only e at the segment's start (from zero) and the sum of delta.
-template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds__(BwdShape<NPL>::W * 64) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
-  constexpr int W = BwdShape<NPL>::W, TT = BwdShape<NPL>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL, NX = STATE ? 2 : 3;
+template <typename T, int NPL, bool STATE, bool GATE, bool WIDE> __global__ __launch_bounds__((BwdShape<NPL, WIDE>::W * 64), (BwdShape<NPL, WIDE>::SIMD)) void ssm_bwd_kernel(w2s_ssm_args a, Plan p) {
+  constexpr int W = BwdShape<NPL, WIDE>::W, TT = BwdShape<NPL, WIDE>::TT, TILE = W * TT, NI = TT / 4, NP = 4 * NPL, NX = STATE ? 2 : 3;
   __shared__ float bc[2][TILE * NP * 2];
   __shared__ float ex[W][NX][64 * NPL];
   __shared__ float carry[2][64 * NPL];   // e in front of a tile, from the first wave of the tile behind
@@ -563,7 +558,7 @@ template <typename T, int NPL, bool STATE, bool GATE> __global__ __launch_bounds
       // The second walk in parts of HALF positions from the last part to the first, so that only a part's states are in registers; h first reaches a
       // part's start without keeping any.
       constexpr int HALF = NPL <= 4 ? TT : NPL == 8 ? 2 : 1, PARTS = TT / HALF, JB = NPL < 4 ? NPL : 4;
-      constexpr bool LATE = NPL <= 4;   // a lane's shares of dB and dC wait in registers for the walk's end, which then has no branch inside
+      constexpr bool LATE = NPL <= 4 && TT > 4;   // a lane's shares of dB and dC wait in registers for the walk's end, which then has no branch inside
       float oB[NI], oG[NI], oY[NI], share[TT];
       forget(gp);
       if (!KEEP) forget(A);
@@ -734,18 +729,12 @@ template <typename T> __global__ __launch_bounds__(256) void ssm_reduce_bc_kerne
     if (s % NP + e < a.N) out[s % NP + e] = (T)o[e];
 }
 
-// gA [D][N], gD, gbias [D]: 64 columns x 16 strided sums over the parts a workgroup, then those 16 in order
+// gA [D][N], gD, gbias [D] from the workgroups' shares
 __global__ __launch_bounds__(1024) void ssm_reduce_a_kernel(w2s_ssm_args a, int nparts, const float* part) {
-  __shared__ float red[16][64];
-  const int64_t per = (int64_t)a.D * (a.N + 2), i = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int row = threadIdx.x >> 6;
-  float v = 0.0f;
-  if (i < per)
-    for (int k = row; k < nparts; k += 16) v += part[k * per + i];
-  red[row][threadIdx.x & 63] = v;
-  __syncthreads();
-  if (row || i >= per) return;
-  for (int k = 1; k < 16; ++k) v += red[k][threadIdx.x];
+  __shared__ float red[64][17];
+  const int64_t C = (int64_t)a.D * (a.N + 2), i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15);
+  const float v = mix_part_sum(part, nparts, C, i, red);
+  if (threadIdx.x >= 16 || i >= C) return;
   const int n = (int)(i % (a.N + 2));
   const int64_t d = i / (a.N + 2);
   if (n < a.N) a.gA[d * a.N + n] = v;
@@ -804,11 +793,8 @@ bool valid(const w2s_ssm_args* a) {
 }
 
 int npl_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
-template <int NPL> constexpr int fwd_tile() { return FwdShape<NPL>::W * FwdShape<NPL>::TT; }
-template <int NPL> constexpr int bwd_tile() { return BwdShape<NPL>::W * BwdShape<NPL>::TT; }
-
-// Segments a sequence is cut into.  Cutting costs a second walk for the end states, so it pays only where the workgroups of whole sequences leave
-// most of the 256 CUs idle.
+// Segments a sequence is cut into.  Cutting costs a second walk for the end states (half of a whole one), so it pays only where the workgroups of whole
+// sequences leave half of the 256 CUs idle or more: then up to two workgroups a CU, of two tiles at least.
 int segments(int64_t blocks, int ntile) {
   if (blocks <= 0 || blocks > 128 || ntile < 4) return 1;
   int64_t n = 512 / blocks;
@@ -817,17 +803,25 @@ int segments(int64_t blocks, int ntile) {
   return n < 2 ? 1 : (int)n;
 }
 
-template <int NPL> Plan plan_of(const w2s_ssm_args* a, bool backward) {
+bool wide(int NPL, int64_t blocks, int nseg) { return NPL <= 4 && nseg == 1 && blocks <= 256; }
+
+template <int NPL> Plan plan_of(const w2s_ssm_args* a, bool backward, bool* is_wide) {
   Plan p{};
-  const int tile = backward ? bwd_tile<NPL>() : fwd_tile<NPL>();
   p.dg = a->D / a->G;
   p.ncb = (p.dg + 15) / 16;
-  p.ntile = (int)(((int64_t)a->L + tile - 1) / tile);
-  p.nseg = segments((int64_t)a->B * a->G * p.ncb, p.ntile);
+  const int64_t blocks = (int64_t)a->B * a->G * p.ncb;
+  auto tiles = [&](int tile) { return (int)(((int64_t)a->L + tile - 1) / tile); };
+  constexpr int ft = FwdShape<NPL, false>::W * FwdShape<NPL, false>::TT, ftw = FwdShape<NPL, true>::W * FwdShape<NPL, true>::TT;
+  constexpr int bt = BwdShape<NPL, false>::W * BwdShape<NPL, false>::TT, btw = BwdShape<NPL, true>::W * BwdShape<NPL, true>::TT;
+  const bool bw = wide(NPL, blocks, segments(blocks, tiles(bt)));
+  p.ck = bw ? btw : bt;
+  p.nck = tiles(p.ck);
+  p.nseg = segments(blocks, tiles(backward ? bt : ft));
+  *is_wide = backward ? bw : wide(NPL, blocks, p.nseg);
+  p.ntile = backward ? p.nck : tiles(*is_wide ? ftw : ft);
   p.tps = (p.ntile + p.nseg - 1) / p.nseg;
   if (p.tps > 0) p.nseg = (p.ntile + p.tps - 1) / p.tps;
   if (p.nseg < 1) p.nseg = 1;
-  p.nck = (int)(((int64_t)a->L + bwd_tile<NPL>() - 1) / bwd_tile<NPL>());
   const int e = esize(a->dtype);
   p.vbc = a->N % 4 == 0 && mix_aligned(a->Bm, a->sB_b, a->sB_l, 4, e) && a->sB_g % 4 == 0 && mix_aligned(a->Cm, a->sC_b, a->sC_l, 4, e) && a->sC_g % 4 == 0;
   if (p.vbc && a->N == 4 * NPL) p.vbc = 2;
@@ -839,39 +833,49 @@ int64_t bc_floats(const w2s_ssm_args* a, const Plan& p, int np) { return (int64_
 int64_t a_floats(const w2s_ssm_args* a, const Plan& p) { return ((int64_t)a->B * p.nseg * a->D * (a->N + 2) + 3) / 4 * 4; }   // (what follows stays 16-byte aligned)
 
 template <int NPL> int64_t ws_floats(const w2s_ssm_args* a, bool backward) {
-  const Plan p = plan_of<NPL>(a, backward);
+  bool w;
+  const Plan p = plan_of<NPL>(a, backward, &w);
   return seg_floats(a, p, 4 * NPL) + (backward ? bc_floats(a, p, 4 * NPL) + a_floats(a, p) : 0);
 }
 
-template <int NPL> int64_t ckpt_floats(const w2s_ssm_args* a) { return (int64_t)a->B * plan_of<NPL>(a, false).nck * a->D * 4 * NPL; }
+template <int NPL> int64_t ckpt_floats(const w2s_ssm_args* a) {
+  bool w;
+  return (int64_t)a->B * plan_of<NPL>(a, false, &w).nck * a->D * 4 * NPL;
+}
 
 template <typename T, int NPL, bool GATE> int scan_fwd(const w2s_ssm_args* a, hipStream_t st) {
-  Plan p = plan_of<NPL>(a, false);
+  bool w;
+  Plan p = plan_of<NPL>(a, false, &w);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
   if (blocks > 0x7fffffff) return W2S_EINVAL;
   if (p.nseg > 1) {
     if (!a->ws) return W2S_EINVAL;
     p.segh = (float*)a->ws;
     p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
-    ssm_fwd_kernel<T, NPL, true, false><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    ssm_fwd_kernel<T, NPL, true, false, false><<<(unsigned)blocks, FwdShape<NPL, false>::W * 64, 0, st>>>(*a, p);
   }
-  ssm_fwd_kernel<T, NPL, false, GATE><<<(unsigned)blocks, FwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+  constexpr bool V = NPL <= 4;
+  if (w) ssm_fwd_kernel<T, NPL, false, GATE, V><<<(unsigned)blocks, FwdShape<NPL, V>::W * 64, 0, st>>>(*a, p);
+  else ssm_fwd_kernel<T, NPL, false, GATE, false><<<(unsigned)blocks, FwdShape<NPL, false>::W * 64, 0, st>>>(*a, p);
   W2S_CHECK_LAUNCH();
   return W2S_OK;
 }
 
 template <typename T, int NPL, bool GATE> int scan_bwd(const w2s_ssm_args* a, hipStream_t st) {
-  Plan p = plan_of<NPL>(a, true);
+  bool w;
+  Plan p = plan_of<NPL>(a, true, &w);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
-  const int64_t rows = (int64_t)a->B * a->L * a->G, nbc = (rows * (2 * NPL) + 255) / 256, na = ((int64_t)a->D * (a->N + 2) + 63) / 64;
+  const int64_t rows = (int64_t)a->B * a->L * a->G, nbc = (rows * (2 * NPL) + 255) / 256, na = ((int64_t)a->D * (a->N + 2) + 15) / 16;
   if (blocks > 0x7fffffff || nbc > 0x7fffffff || na > 0x7fffffff) return W2S_EINVAL;
   p.part_bc = (float*)a->ws;
   p.part_a = p.part_bc + bc_floats(a, p, 4 * NPL);
   p.segh = p.part_a + a_floats(a, p);
   p.segs = p.segh + (int64_t)a->B * p.nseg * a->D * 4 * NPL;
   if (blocks) {
-    if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true, GATE><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
-    ssm_bwd_kernel<T, NPL, false, GATE><<<(unsigned)blocks, BwdShape<NPL>::W * 64, 0, st>>>(*a, p);
+    constexpr bool V = NPL <= 4;
+    if (p.nseg > 1) ssm_bwd_kernel<T, NPL, true, GATE, false><<<(unsigned)blocks, BwdShape<NPL, false>::W * 64, 0, st>>>(*a, p);
+    if (w) ssm_bwd_kernel<T, NPL, false, GATE, V><<<(unsigned)blocks, BwdShape<NPL, V>::W * 64, 0, st>>>(*a, p);
+    else ssm_bwd_kernel<T, NPL, false, GATE, false><<<(unsigned)blocks, BwdShape<NPL, false>::W * 64, 0, st>>>(*a, p);
   }
   if (nbc) ssm_reduce_bc_kernel<T><<<(unsigned)nbc, 256, 0, st>>>(*a, p.ncb, 4 * NPL, p.part_bc);
   ssm_reduce_a_kernel<<<(unsigned)na, 1024, 0, st>>>(*a, a->B * p.nseg, p.part_a);
