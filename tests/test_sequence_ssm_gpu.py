@@ -1,0 +1,111 @@
+"""The state space sequence mixer inside the framework: against a 64-bit statement, one epoch at a time, its gradients, a train step.
+
+The walker's matrix products run in split bf16 (relative error <= 2^-16 a product, the library's arithmetic class), so features are compared at 1e-3 of
+the largest and gradients at 2e-3 relative L2 -- the bars that the generic path's other tests use."""
+import pytest
+import torch
+
+import wav2sleep_amd as W
+from tests import mixer_reference as R
+
+pytestmark = pytest.mark.gpu
+
+
+def mixer(F=64, layers=2, seed=0, **kw):
+    torch.manual_seed(seed)
+    m = W.SequenceSSM(F, num_layers=layers, state_dim=16, expand=2, **kw)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(0.02 * torch.randn_like(p))
+    return m.to('cuda')
+
+
+def reference(m, x):
+    """[B, S, F] in 64 bits with autograd through plain torch operations -> features, {name: parameter leaf}"""
+    P = {k: v.detach().double().requires_grad_(True) for k, v in m.named_parameters()}
+    h, res, N, r = x.double(), None, m.state_dim, m.dt_rank
+    F = torch.nn.functional
+
+    def norm(t, w):
+        return t / torch.sqrt(t.pow(2).mean(-1, keepdim=True) + m.norm_eps) * w
+    for i in range(m.num_layers):
+        p = lambda k: P[f'layers.{i}.{k}']   # noqa: E731, B023
+        res = h if res is None else h + res
+        n = norm(res, p('norm_weight'))
+        u, z = n @ p('in_proj.weight').t(), n @ p('gate_proj.weight').t()
+        pad = F.pad(u.transpose(1, 2), (m.kernel_size - 1, 0))
+        u = F.silu(F.conv1d(pad, p('conv_weight')[:, None], p('conv_bias'), groups=u.shape[-1])).transpose(1, 2)
+        dbc = u @ p('x_proj.weight').t()
+        delta = F.softplus(dbc[..., :r] @ p('dt_proj.weight').t() + p('dt_bias'))
+        A = -torch.exp(p('A_log'))
+        st, ys = torch.zeros(*u.shape[::2], N, device=x.device, dtype=torch.float64), []
+        for t in range(u.shape[1]):
+            st = torch.exp(delta[:, t, :, None] * A) * st + (delta[:, t] * u[:, t])[..., None] * dbc[:, t, None, r:r + N]
+            ys.append((st * dbc[:, t, None, r + N:]).sum(-1))
+        y = (torch.stack(ys, 1) + p('D') * u) * F.silu(z)
+        h = y @ p('out_proj.weight').t()
+    return norm(h + res, P['norm_weight']), P
+
+
+@pytest.mark.parametrize('shape', [(1, 1), (3, 17), (2, 130)], ids=str)
+def test_features_and_steps(shape):
+    m = mixer().eval()
+    x = torch.randn(*shape, 64, device='cuda')
+    want = reference(m, x)[0].detach()
+    got = m(x)
+    size = float(want.abs().max())
+    assert float((got - want).abs().max()) <= 1e-3 * size
+    state = m.init_state(shape[0])
+    for t in range(shape[1]):
+        y = m.step(x[:, t], state)
+        assert float((y - want[:, t]).abs().max()) <= 1e-3 * size, t
+
+
+def test_later_epochs_do_not_reach_earlier_ones():
+    m = mixer().eval()
+    x = torch.randn(2, 60, 64, device='cuda')
+    a = m(x)
+    x[:, 40:] += 1.0
+    b = m(x)
+    assert torch.equal(a[:, :40], b[:, :40]) and not torch.equal(a[:, 40:], b[:, 40:])
+
+
+def test_gradients_of_the_walkers_tape():
+    from wav2sleep_amd.generic import GenericForward
+    m = mixer().train()
+    x = torch.randn(2, 45, 64, device='cuda')
+    g = torch.randn(2, 45, 64, device='cuda')
+    gf = GenericForward(training=True, seed=1, grad=True)
+    with torch.no_grad():
+        out = gf.sequence_ssm(m, x)
+        got = gf.backward(out, g)
+    want, P = reference(m, x)
+    grads = dict(zip(P, torch.autograd.grad((want * g.double()).sum(), list(P.values()))))
+    named = dict(m.named_parameters())
+    assert set(got) == set(named.values())
+    for k, p in named.items():
+        rel = float((got[p].double() - grads[k]).norm() / grads[k].norm())
+        assert rel <= 2e-3, (k, rel)
+
+
+def test_model_trains_with_it(tmp_path):
+    """the whole model: a train step through SleepModule moves every parameter, its state dict comes back through load_model with the same logits"""
+    torch.manual_seed(0)
+    enc = W.SignalEncoders({'THX': 'THX', 'ECG': 'ECG'}, 64, 'gelu', norm='instance', chunk_causal=False, max_channels=32)
+    model = W.Wav2Sleep(enc, W.MultiModalAttentionEmbedder(64, layers=1, nhead=4, dim_ff=64), W.SequenceSSM(64, num_layers=1, state_dim=8, expand=1), 4).to('cuda')
+    x = {'THX': torch.randn(2, 256 * 6, device='cuda'), 'ECG': torch.randn(2, 1024 * 6, device='cuda')}
+    y = torch.randint(0, 4, (2, 6), device='cuda').float()
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    mod = W.SleepModule(model, num_classes=4, lr=1e-3)
+    loss = mod.training_step((x, y))
+    assert torch.isfinite(torch.as_tensor(float(loss)))
+    still = [k for k, v in model.state_dict().items() if torch.equal(v, before[k]) and v.is_floating_point()]
+    assert not still, still
+    model.eval()
+    with torch.no_grad():
+        a = model(x)
+    W.save_model(str(tmp_path), model)
+    with torch.no_grad():
+        assert torch.equal(W.load_model(str(tmp_path), device='cuda')(x), a)
+    out = mod.validation_step((x, y))
+    assert all(torch.isfinite(torch.as_tensor(float(v))) for v in out.values())

@@ -15,6 +15,7 @@ import torch
 import yaml
 
 from . import ppgnet as _ppg
+from . import ssm as _ssm
 from . import wav2sleep as _w
 
 _TARGETS = {
@@ -22,6 +23,7 @@ _TARGETS = {
     'wav2sleep.models.wav2sleep.SignalEncoders': _w.SignalEncoders,
     'wav2sleep.models.wav2sleep.MultiModalAttentionEmbedder': _w.MultiModalAttentionEmbedder,
     'wav2sleep.models.wav2sleep.SequenceCNN': _w.SequenceCNN,
+    'wav2sleep_amd.SequenceSSM': _ssm.SequenceSSM,   # (no counterpart in the reference)
     'wav2sleep.models.ppgnet.SleepPPGNet': _ppg.SleepPPGNet,   # scripts/config/model/ppgnet.yaml
 }
 

@@ -767,6 +767,83 @@ class GenericForward:
             x = self.dilated_block(block, x)
         return x
 
+    # ------------------------------------------------------------------ state space mixer (ssm.py)
+    def _add_norm(self, x, res, wp, eps):
+        """r = x + res, y = RMS norm of r over rows [rows, C] in one launch -> (y, r); res None: r is x"""
+        w = wp.detach()
+        y = torch.empty_like(x)
+        r = x if res is None else torch.empty_like(x)
+        rstd = torch.empty(x.shape[0], device=x.device, dtype=torch.float32) if self.grad else None
+        lib.add_norm_fwd(x, w, y, eps, res=res, r=None if res is None else r, rstd=rstd)
+        if res is not None:
+            self._rec(r, (x, res), lambda g: (g, g), share='all')
+
+        def bw(g, acc=None):   # acc: the gradient that r already has as the next residual, added in the same launch
+            gx = acc if acc is not None else torch.empty_like(r)
+            gw = torch.empty_like(w)
+            lib.add_norm_bwd(r, w, rstd, g.contiguous(), acc, gx, gw, eps)
+            self._pgrad(wp, gw)
+            return (gx,)
+        self._rec(y, (r,), bw, acc_ok=True)
+        return y, r
+
+    def _short_conv(self, x, wp, bp):
+        w, b = wp.detach(), bp.detach()
+        y = torch.empty_like(x)
+        lib.short_conv_fwd(x, w, b, y)
+
+        def bw(g):
+            gx, gw, gb = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+            lib.short_conv_bwd(x, w, b, g.contiguous(), gx, gw, gb)
+            self._pgrad(wp, gw)
+            self._pgrad(bp, gb)
+            return (gx,)
+        self._rec(y, (x,), bw)
+        return y
+
+    def _columns(self, t, a, b):
+        """columns a:b of [rows, C], contiguous (plumbing on the small projection)"""
+        o = t[:, a:b].contiguous()
+        self._rec(o, (t,), lambda g: (nn.functional.pad(g, (a, t.shape[1] - b)),))
+        return o
+
+    def _ssm_scan(self, u, dt, Bm, Cm, z, layer):
+        """selective scan of u [B, S, E] with B, C [B, S, 1, N], gated by z"""
+        A, D, bias = -torch.exp(layer.A_log.detach()), layer.D.detach(), layer.dt_bias.detach()
+        y = torch.empty_like(u)
+        ckpt = lib.ssm_scan_fwd(u, dt, A, Bm, Cm, D, z, bias, y, keep=self.grad)
+
+        def bw(g):
+            e = torch.empty_like
+            gu, gdt, gz, gB, gC, gA, gD, gb = e(u), e(dt), e(z), e(Bm), e(Cm), e(A), e(D), e(bias)
+            lib.ssm_scan_bwd(u, dt, A, Bm, Cm, D, z, bias, ckpt, g.contiguous(), gu=gu, gdt=gdt, gz=gz, gB=gB, gC=gC, gA=gA, gD=gD, gbias=gb)
+            self._pgrad(layer.A_log, gA * A)   # A = -exp(A_log)
+            self._pgrad(layer.D, gD)
+            self._pgrad(layer.dt_bias, gb)
+            return (gu, gdt, gB, gC, gz)
+        self._rec(y, (u, dt, Bm, Cm, z), bw)
+        return y
+
+    def sequence_ssm(self, mod, x_BSF):
+        """SequenceSSM.forward: [B, S, F] -> [B, S, F]"""
+        x = x_BSF if (x_BSF.is_contiguous() and x_BSF.dtype == torch.float32) else x_BSF.contiguous().float()
+        B, S, F_ = x.shape
+        if F_ != mod.feature_dim:
+            raise ValueError(f'Feature dimension {F_} does not match {mod.feature_dim=}.')
+        R, E, N, r = B * S, mod.inner_dim, mod.state_dim, mod.dt_rank
+        h, res = self._view(x, R, F_), None
+        for layer in mod.layers:
+            n, res = self._add_norm(h, res, layer.norm_weight, mod.norm_eps)
+            u = self._short_conv(self._view(self.linear(n, layer.in_proj.weight, None), B, S, E), layer.conv_weight, layer.conv_bias)
+            z = self._view(self.linear(n, layer.gate_proj.weight, None), B, S, E)
+            dbc = self.linear(self._view(u, R, E), layer.x_proj.weight, None)
+            dt = self._view(self.linear(self._columns(dbc, 0, r), layer.dt_proj.weight, None), B, S, E)
+            Bm, Cm = (self._view(self._columns(dbc, r + q * N, r + (q + 1) * N), B, S, 1, N) for q in (0, 1))
+            y = self._ssm_scan(u, dt, Bm, Cm, z, layer)
+            h = self._dropout_(self.linear(self._view(y, R, E), layer.out_proj.weight, None), mod.dropout_p)
+        y, _ = self._add_norm(h, res, mod.norm_weight, mod.norm_eps)
+        return self._view(y, B, S, F_)
+
     def classifier(self, lin: nn.Linear, x_BSF):
         B, S, F_ = x_BSF.shape
         nc = lin.out_features
@@ -795,7 +872,9 @@ class GenericForward:
         """Wav2Sleep.forward (wav2sleep.py:48-67)."""
         z = self.signal_encoders(model.signal_encoders, x)
         m = self.mixer(model.epoch_mixer, z)
-        s = self.sequence_cnn(model.sequence_mixer, m)
+        from .ssm import SequenceSSM
+        mix = self.sequence_ssm if isinstance(model.sequence_mixer, SequenceSSM) else self.sequence_cnn
+        s = mix(model.sequence_mixer, m)
         return self.classifier(model.classifier, s)
 
     def ppgnet(self, model, x_BT) -> torch.Tensor:

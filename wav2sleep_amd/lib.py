@@ -803,5 +803,69 @@ def load_torch_ops():
     return _w2s_torch
 
 
+def _io(t):
+    return IO_DTYPES[t.dtype]
+
+
+def add_norm_fwd(x, w, y, eps, res=None, r=None, rstd=None):
+    """y = RMS norm of x (+ res, whose sum goes to r) over the rows of contiguous [rows, C] tensors; rstd [rows] for the backward"""
+    rows, Cc = x.shape
+    a = AddNormArgs(x=_p(x), res=_p(res), w=_f(w), y=_p(y), r=_p(r), rstd=_f(rstd), rows=rows, ldx=Cc, ldres=Cc, C=Cc, dtype=_io(x), rdtype=_io(x if res is None else res), eps=eps)
+    _chk(load().w2s_add_norm_fwd(C.byref(a), _stream()), 'w2s_add_norm_fwd')
+
+
+def add_norm_bwd(r, w, rstd, gy, gr, gx, gw, eps):
+    """gx = gradient of the fp32 sum r (+ gr, which may be gx itself), gw = gradient of w"""
+    rows, Cc = r.shape
+    a = AddNormArgs(res=_f(r), w=_f(w), rstd=_f(rstd), gy=_f(gy), gr=_f(gr), gx=_f(gx), gw=_f(gw), rows=rows, ldres=Cc, ldgy=Cc, ldgr=Cc, C=Cc, eps=eps)
+    n = load().w2s_add_norm_part(C.byref(a))
+    part = torch.empty(max(1, n), device=r.device, dtype=torch.float32)
+    a.part = _f(part)
+    _chk(load().w2s_add_norm_bwd(C.byref(a), _stream()), 'w2s_add_norm_bwd')
+
+
+def _short_conv_args(x, w, bias, act, **kw):
+    B, L, D = x.shape
+    return ShortConvArgs(x=_p(x), w=_f(w), bias=_f(bias), B=B, L=L, D=D, K=w.shape[1], dtype=_io(x), act=act, sx_b=x.stride(0), sx_l=x.stride(1), **kw)
+
+
+def short_conv_fwd(x, w, bias, y, act=1, state_out=None):
+    """depthwise causal convolution of x [B, L, D] with w [D, K] (+ SiLU: act 1), from zeros"""
+    a = _short_conv_args(x, w, bias, act, y=_p(y), state_out=_p(state_out))
+    _chk(load().w2s_short_conv_fwd(C.byref(a), _stream()), 'w2s_short_conv_fwd')
+
+
+def short_conv_bwd(x, w, bias, gy, gx, gw, gbias, act=1):
+    a = _short_conv_args(x, w, bias, act, gy=_p(gy), gx=_p(gx), gw=_f(gw), gbias=_f(gbias), sg_b=gy.stride(0), sg_l=gy.stride(1))
+    part = torch.empty(max(1, load().w2s_short_conv_part(C.byref(a))), device=x.device, dtype=torch.float32)
+    a.part = _f(part)
+    _chk(load().w2s_short_conv_bwd(C.byref(a), _stream()), 'w2s_short_conv_bwd')
+
+
+def _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, **kw):
+    B, L, Dc = u.shape
+    return SsmArgs(u=_p(u), dt=_p(dt), z=_p(z), Bm=_p(Bm), Cm=_p(Cm), A=_f(A), Dp=_f(D), dt_bias=_f(dt_bias), su_b=u.stride(0), su_l=u.stride(1), sdt_b=dt.stride(0), sdt_l=dt.stride(1),
+                   sz_b=0 if z is None else z.stride(0), sz_l=0 if z is None else z.stride(1), sB_b=Bm.stride(0), sB_l=Bm.stride(1), sB_g=Bm.stride(2),
+                   sC_b=Cm.stride(0), sC_l=Cm.stride(1), sC_g=Cm.stride(2), B=B, L=L, D=Dc, N=A.shape[1], G=Bm.shape[2], dtype=_io(u), softplus=1, **kw)
+
+
+def ssm_scan_fwd(u, dt, A, Bm, Cm, D, z, dt_bias, y, keep=False, h_out=None):
+    """selective scan of [B, L, D] from a zero state; keep: returns what ssm_scan_bwd starts from"""
+    a = _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, y=_p(y), h_out=_f(h_out))
+    ckpt = torch.empty(max(1, load().w2s_ssm_ckpt(C.byref(a))), device=u.device, dtype=torch.float32) if keep else None
+    ws = torch.empty(max(1, load().w2s_ssm_ws(C.byref(a), 0)), device=u.device, dtype=torch.uint8)
+    a.ckpt, a.ws = _f(ckpt), _p(ws)
+    _chk(load().w2s_ssm_scan_fwd(C.byref(a), _stream()), 'w2s_ssm_scan_fwd')
+    return ckpt
+
+
+def ssm_scan_bwd(u, dt, A, Bm, Cm, D, z, dt_bias, ckpt, gy, *, gu, gdt, gz, gB, gC, gA, gD, gbias):
+    a = _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, ckpt=_f(ckpt), gy=_p(gy), gu=_p(gu), gdt=_p(gdt), gz=_p(gz), gB=_p(gB), gC=_p(gC), gA=_f(gA), gD=_f(gD), gbias=_f(gbias),
+                       sg_b=gy.stride(0), sg_l=gy.stride(1))
+    ws = torch.empty(max(1, load().w2s_ssm_ws(C.byref(a), 1)), device=u.device, dtype=torch.uint8)
+    a.ws = _p(ws)
+    _chk(load().w2s_ssm_scan_bwd(C.byref(a), _stream()), 'w2s_ssm_scan_bwd')
+
+
 def version() -> str:
     return load().w2s_version().decode()

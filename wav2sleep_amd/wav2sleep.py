@@ -534,7 +534,7 @@ class Wav2Sleep(_HandWritten, nn.Module):
             'epoch_mixer': {'_target_': t + 'MultiModalAttentionEmbedder', 'feature_dim': em.feature_dim, 'dropout': em.dropout_p,
                             'activation': 'gelu', 'layers': em.num_layers, 'dim_ff': em.dim_ff, 'nhead': em.nhead,
                             'register_tokens': em.num_register_tokens},
-            'sequence_mixer': {'_target_': t + 'SequenceCNN', 'feature_dim': self.feature_dim, 'dropout': sm.dropout_p, 'activation': 'gelu',
+            'sequence_mixer': sm.config_dict() if hasattr(sm, 'config_dict') else {'_target_': t + 'SequenceCNN', 'feature_dim': self.feature_dim, 'dropout': sm.dropout_p, 'activation': 'gelu',
                                'norm': 'layer', 'causal': bool(sm.causal), 'num_layers': sm.num_layers, 'kernel_size': sm.kernel_size,
                                'num_dilations': sm.num_dilations},
         }
