@@ -1,10 +1,29 @@
 // Root-mean-square norm with the residual's addition: r = x + res, y = r rstd w, rstd = 1 / sqrt(mean(r^2) + eps), y in 16 / 32 bits or in e4m3
 // with one scale a row.  Three or four elements moved per element and five flops: bound by HBM, so a row is read once and lives in registers
-// (G lanes x NV vectors) between the sum of squares and the product; only rows beyond 256 lanes x 8 vectors, and widths or pointers that
-// no vector access fits, are read twice (the second time from L2) by the looped kernel.  The sum is fp32 and y comes from it before r is rounded.
+// (G lanes x NV vectors) between the sum of squares and the product; only rows beyond 256 lanes x 8 vectors (4 in the
+// backward) are read twice, the second time from L2, by the looped kernel.  Any width, stride and alignment takes the same accesses.  The sum is fp32 and y comes from it before r is rounded.
 #include "mix_io.h"
 
 namespace {
+
+// VEC columns from c on of a row of C; behind the row's end zeros / nothing
+template <typename T, int VEC> __device__ __forceinline__ void load_cols(const T* row, int c, int C, float* v) {
+  if (c + VEC <= C) {
+    mix_gload<T, VEC>(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = c + i < C ? (float)row[c + i] : 0.0f;
+  }
+}
+template <typename T, int VEC> __device__ __forceinline__ void store_cols(T* row, int c, int C, const float* v) {
+  if (c + VEC <= C) {
+    mix_gstore<T, VEC>(row + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (c + i < C) row[c + i] = (T)v[i];
+  }
+}
 
 constexpr float kFp8Max = 448.0f;   // largest finite e4m3 value
 
@@ -25,19 +44,24 @@ template <int G, bool MAX> __device__ __forceinline__ float row_reduce(float v, 
   }
 }
 
-template <int N> __device__ __forceinline__ void store_fp8(uint8_t* p, const float* v) {   // v within +-448 or NaN
-  if constexpr (N == 1) {
-    *p = (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[0], 0, false) & 0xff);
-  } else {
-    static_assert(N % 4 == 0, "four codes a word");
-    uint32_t w[N / 4];
+__device__ __forceinline__ uint8_t fp8_code(float v) { return (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(v, v, 0, false) & 0xff); }
+
+template <int N> __device__ __forceinline__ void store_fp8(uint8_t* row, int c, int C, const float* v) {   // v within +-448 or NaN
+  static_assert(N == 4 || N == 8, "words of four codes");
+  if (c + N <= C) {
+    typedef uint32_t U __attribute__((ext_vector_type(N / 4)));
+    typedef U UU __attribute__((aligned(1)));
+    U w;
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
+      const int q = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i], v[4 * i + 1], 0, false);
       w[i] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * i + 2], v[4 * i + 3], q, true);
     }
-    if constexpr (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
-    else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<UU*>(row + c) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (c + i < C) row[c + i] = fp8_code(v[i]);
   }
 }
 
@@ -61,19 +85,14 @@ template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ 
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * G + lane) * VEC;
-    if (c < C) {
-      mix_load<T, VEC>(x + c, v[j]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
-    }
+    load_cols<T, VEC>(x, c, C, v[j]);
   }
   if (res) {
     float q[NV][VEC];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * G + lane) * VEC;
-      if (c < C) mix_load<RT, VEC>(res + c, q[j]);
+      load_cols<RT, VEC>(res, c, C, q[j]);
     }
     RT* r = (RT*)a.r + row * C;
 #pragma unroll
@@ -82,7 +101,7 @@ template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ 
       if (c < C) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j][i] += q[j][i];
-        mix_store<RT, VEC>(r + c, v[j]);
+        store_cols<RT, VEC>(r, c, C, v[j]);
       }
     }
   }
@@ -99,13 +118,13 @@ template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ 
     const int c = (j * G + lane) * VEC;
     if (c < C) {
       float w[VEC];
-      mix_load<float, VEC>(a.w + c, w);
+      load_cols<float, VEC>(a.w, c, C, w);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[j][i] *= rstd * w[i];
         if (FP8) top = v[j][i] != v[j][i] || top != top ? __builtin_nanf("") : fmaxf(top, __builtin_fabsf(v[j][i]));
       }
-      if (!FP8) mix_store<T, VEC>((T*)a.y + row * C + c, v[j]);
+      if (!FP8) store_cols<T, VEC>((T*)a.y + row * C, c, C, v[j]);
     }
   }
   if (FP8) {
@@ -120,13 +139,13 @@ template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ 
       if (c < C) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[j][i] = to_fp8_range(v[j][i], scale);
-        store_fp8<VEC>((uint8_t*)a.y + row * C + c, v[j]);
+        store_fp8<VEC>((uint8_t*)a.y + row * C, c, C, v[j]);
       }
     }
   }
 }
 
-// any width, any alignment: a workgroup per row, one element a lane, the row's sum formed again in every pass
+// rows too wide for registers: a workgroup per row, one element a lane, the row's sum formed again in every pass
 template <typename T, typename RT, bool FP8> __global__ __launch_bounds__(256) void add_norm_fwd_loop_kernel(w2s_add_norm_args a) {
   __shared__ float red[4];
   const int C = a.C;
@@ -157,8 +176,7 @@ template <typename T, typename RT, bool FP8> __global__ __launch_bounds__(256) v
   const float scale = fp8_scale(top);
   if (threadIdx.x == 0) a.scale[row] = scale;
   for (int c = threadIdx.x; c < C; c += 256) {
-    const float q = to_fp8_range(sum_at(c) * (rstd * a.w[c]), scale);
-    store_fp8<1>((uint8_t*)a.y + row * C + c, &q);
+    ((uint8_t*)a.y)[row * C + c] = fp8_code(to_fp8_range(sum_at(c) * (rstd * a.w[c]), scale));
   }
 }
 
@@ -175,7 +193,7 @@ template <typename T, typename RT, int VEC, int G, int NV> __global__ __launch_b
     const int c = (j * G + lane) * VEC;
 #pragma unroll
     for (int i = 0; i < VEC; ++i) gw[j][i] = w[j][i] = 0.0f;
-    if (c < C) mix_load<float, VEC>(a.w + c, w[j]);
+    load_cols<float, VEC>(a.w, c, C, w[j]);
   }
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
     const int64_t row = r0 + threadIdx.x / G;
@@ -187,14 +205,14 @@ template <typename T, typename RT, int VEC, int G, int NV> __global__ __launch_b
 #pragma unroll
       for (int i = 0; i < VEC; ++i) n[j][i] = g[j][i] = 0.0f;
       if (on && c < C) {
-        if (a.x) mix_load<T, VEC>((const T*)a.x + row * a.ldx + c, n[j]);
+        if (a.x) load_cols<T, VEC>((const T*)a.x + row * a.ldx, c, C, n[j]);
         if (a.res) {
           float q[VEC];
-          mix_load<RT, VEC>((const RT*)a.res + row * a.ldres + c, q);
+          load_cols<RT, VEC>((const RT*)a.res + row * a.ldres, c, C, q);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) n[j][i] += q[i];
         }
-        if (a.gy) mix_load<T, VEC>((const T*)a.gy + row * a.ldgy + c, g[j]);
+        if (a.gy) load_cols<T, VEC>((const T*)a.gy + row * a.ldgy, c, C, g[j]);
       }
     }
     const float rstd = on ? a.rstd[row] : 0.0f;
@@ -216,11 +234,11 @@ template <typename T, typename RT, int VEC, int G, int NV> __global__ __launch_b
         float o[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] = 0.0f;
-        if (a.gr) mix_load<RT, VEC>((const RT*)a.gr + row * a.ldgr + c, o);
+        if (a.gr) load_cols<RT, VEC>((const RT*)a.gr + row * a.ldgr, c, C, o);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] += rstd * __builtin_fmaf(-n[j][i], m, g[j][i]);
-        if (a.gx) mix_store<T, VEC>((T*)a.gx + row * C + c, o);
-        if (a.gres) mix_store<RT, VEC>((RT*)a.gres + row * C + c, o);
+        if (a.gx) store_cols<T, VEC>((T*)a.gx + row * C, c, C, o);
+        if (a.gres) store_cols<RT, VEC>((RT*)a.gres + row * C, c, C, o);
       }
     }
   }
@@ -230,7 +248,7 @@ template <typename T, typename RT, int VEC, int G, int NV> __global__ __launch_b
   for (int j = 0; j < NV; ++j) {
     if constexpr (G == 256) {
       const int c = (j * G + lane) * VEC;
-      if (c < C) mix_store<float, VEC>(part + c, gw[j]);
+      store_cols<float, VEC>(part, c, C, gw[j]);
     } else {
       __syncthreads();
 #pragma unroll
@@ -289,17 +307,6 @@ bool valid(const w2s_add_norm_args* a) {
          (a->rdtype == a->dtype || a->rdtype == W2S_F32);
 }
 
-// elements a lane's access: 16 bytes of T where widths, rows and pointers allow, else 1
-int vector_of(const w2s_add_norm_args* a) {
-  const int v = 16 / esize(a->dtype);
-  if (a->C % v || a->ldx % v || a->ldres % v || a->ldgy % v || a->ldgr % v) return 1;
-  const void* ps[] = {a->x, a->res, a->w, a->r, a->gy, a->gr, a->gx, a->gres};
-  for (const void* p : ps)
-    if ((uintptr_t)p % 16) return 1;
-  if ((uintptr_t)a->y % (a->fp8 ? 8 : 16)) return 1;
-  return v;
-}
-
 // workgroups of the backward: enough for 8 waves a SIMD quad on every CU, at most one per row group
 int bwd_blocks(const w2s_add_norm_args* a) {
   const int64_t n = a->rows < 1 ? 1 : a->rows;
@@ -309,8 +316,7 @@ int bwd_blocks(const w2s_add_norm_args* a) {
 template <typename T, typename RT, int VEC, int G, int NV> int go(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
   const int64_t groups = (a->rows + 256 / G - 1) / (256 / G);
   if (bwd) {
-    const int nb = bwd_blocks(a);
-    add_norm_bwd_kernel<T, RT, VEC, G, NV><<<nb, 256, 0, st>>>(*a);
+    if constexpr (NV <= 4) add_norm_bwd_kernel<T, RT, VEC, G, NV><<<bwd_blocks(a), 256, 0, st>>>(*a);
   } else if (a->fp8) {
     add_norm_fwd_kernel<T, RT, true, VEC, G, NV><<<(unsigned)groups, 256, 0, st>>>(*a);
   } else {
@@ -321,7 +327,7 @@ template <typename T, typename RT, int VEC, int G, int NV> int go(const w2s_add_
 
 template <typename T, typename RT> int by_width(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
   constexpr int V = 16 / (int)sizeof(T);
-  const int units = vector_of(a) == V ? a->C / V : 1 << 30;   // lanes' accesses a row
+  const int units = (a->C + V - 1) / V;   // lanes' accesses of 16 bytes (of T) a row
   if (units <= 16) return go<T, RT, V, 16, 1>(a, bwd, st);
   if (units <= 32) return go<T, RT, V, 32, 1>(a, bwd, st);
   if (units <= 64) return go<T, RT, V, 64, 1>(a, bwd, st);
@@ -329,6 +335,7 @@ template <typename T, typename RT> int by_width(const w2s_add_norm_args* a, bool
   if (units <= 256) return go<T, RT, V, 256, 1>(a, bwd, st);
   if (units <= 512) return go<T, RT, V, 256, 2>(a, bwd, st);
   if (units <= 1024) return go<T, RT, V, 256, 4>(a, bwd, st);
+  if (units <= 2048 && !bwd) return go<T, RT, V, 256, 8>(a, bwd, st);   // (the backward keeps four such rows: it would spill)
   if (bwd) {
     add_norm_bwd_loop_kernel<T, RT><<<bwd_blocks(a), 256, 0, st>>>(*a);
   } else if (a->fp8) {

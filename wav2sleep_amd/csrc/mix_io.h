@@ -10,37 +10,43 @@ typedef __bf16 bf16_t;
 template <typename T, int N> struct mix_vec { typedef T type __attribute__((ext_vector_type(N))); };
 template <typename T> struct mix_vec<T, 1> { typedef T type; };
 
-// N elements as floats; p is aligned to N * sizeof(T) (at most 16 bytes a load)
-template <typename T, int N> __device__ __forceinline__ void mix_load(const T* p, float* v) {
+// N elements as floats.  mix_load / mix_store: p is aligned to N * sizeof(T) (LDS, the library's own scratch memory).  mix_gload / mix_gstore: global memory at
+// any element -- gfx950 takes wide global accesses at any address, so rows of odd width, slices of wider rows and offset pointers are read as wide as others.
+template <typename T, int N, size_t ALIGN> __device__ __forceinline__ void mix_load_at(const T* p, float* v) {
   constexpr int E = 16 / (int)sizeof(T);
   if constexpr (N > E) {
-    mix_load<T, E>(p, v);
-    mix_load<T, N - E>(p + E, v + E);
+    mix_load_at<T, E, ALIGN>(p, v);
+    mix_load_at<T, N - E, ALIGN>(p + E, v + E);
   } else if constexpr (N == 1) {
     v[0] = (float)*p;
   } else {
     typedef typename mix_vec<T, N>::type V;
-    const V r = *reinterpret_cast<const V*>(p);
+    typedef V U __attribute__((aligned(ALIGN ? ALIGN : N * sizeof(T))));
+    const V r = *reinterpret_cast<const U*>(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)r[i];
   }
 }
-
-template <typename T, int N> __device__ __forceinline__ void mix_store(T* p, const float* v) {
+template <typename T, int N, size_t ALIGN> __device__ __forceinline__ void mix_store_at(T* p, const float* v) {
   constexpr int E = 16 / (int)sizeof(T);
   if constexpr (N > E) {
-    mix_store<T, E>(p, v);
-    mix_store<T, N - E>(p + E, v + E);
+    mix_store_at<T, E, ALIGN>(p, v);
+    mix_store_at<T, N - E, ALIGN>(p + E, v + E);
   } else if constexpr (N == 1) {
     *p = (T)v[0];
   } else {
     typedef typename mix_vec<T, N>::type V;
+    typedef V U __attribute__((aligned(ALIGN ? ALIGN : N * sizeof(T))));
     V r;
 #pragma unroll
     for (int i = 0; i < N; ++i) r[i] = (T)v[i];
-    *reinterpret_cast<V*>(p) = r;
+    *reinterpret_cast<U*>(p) = r;
   }
 }
+template <typename T, int N> __device__ __forceinline__ void mix_load(const T* p, float* v) { mix_load_at<T, N, 0>(p, v); }
+template <typename T, int N> __device__ __forceinline__ void mix_store(T* p, const float* v) { mix_store_at<T, N, 0>(p, v); }
+template <typename T, int N> __device__ __forceinline__ void mix_gload(const T* p, float* v) { mix_load_at<T, N, sizeof(T)>(p, v); }
+template <typename T, int N> __device__ __forceinline__ void mix_gstore(T* p, const float* v) { mix_store_at<T, N, sizeof(T)>(p, v); }
 
 // 1 / (1 + e^-x); e^-x may overflow to inf (-> 0) and a NaN stays one
 __device__ __forceinline__ float mix_sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x)); }
@@ -93,8 +99,4 @@ __device__ __forceinline__ float mix_part_sum(const float* part, int nparts, int
     if (r < h) red[r][c] = v += red[r + h][c];
   }
   return v;
-}
-
-static inline bool mix_aligned(const void* p, int64_t s0, int64_t s1, int vec, int esize) {   // base and both strides allow vec-element accesses
-  return ((uintptr_t)p % (size_t)(vec * esize)) == 0 && s0 % vec == 0 && s1 % vec == 0;
 }

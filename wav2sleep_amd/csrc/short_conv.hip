@@ -14,9 +14,9 @@ struct Shape { int ncg, cx, ty, ncgb, nchb, L, D, runs; };   // runs: how many r
 template <typename T, int VEC, int K>
 __device__ __forceinline__ void full_row(const T* x, int64_t sl, const T* state, int D, int r, int n, float* v) {
   if (r >= K - 1) {
-    if (r - (K - 1) < n) { mix_load<T, VEC>(x + (int64_t)(r - (K - 1)) * sl, v); return; }
+    if (r - (K - 1) < n) { mix_gload<T, VEC>(x + (int64_t)(r - (K - 1)) * sl, v); return; }
   } else if (r >= 0 && state) {
-    mix_load<T, VEC>(state + (int64_t)r * D, v);
+    mix_gload<T, VEC>(state + (int64_t)r * D, v);
     return;
   }
 #pragma unroll
@@ -26,18 +26,31 @@ __device__ __forceinline__ void full_row(const T* x, int64_t sl, const T* state,
 // A workgroup's weights through LDS: K consecutive floats a channel in memory are one 128-byte line a lane, which as a vector load costs a wave 64 cache
 // lines an instruction; staged [tap][channel] they are read once, coalesced, by the workgroup.  (The step has one position to spend them on: load_weights.)
 template <int VEC, int K> struct Weights {
-  float w[K][64 * VEC], b[64 * VEC];
+  float w[K][64 * VEC + 4], b[64 * VEC + 4];
   __device__ __forceinline__ void stage(const float* gw, const float* gb, int c0, int nc) {   // channels c0 .. c0 + nc - 1 of the tensor's D
     for (int i = threadIdx.x; i < nc * K; i += 256) w[i % K][i / K] = gw[(int64_t)c0 * K + i];
     for (int i = threadIdx.x; i < nc; i += 256) b[i] = gb ? gb[c0 + i] : 0.0f;
     __syncthreads();
   }
-  __device__ __forceinline__ void get(int lane, float (*wk)[VEC], float* bk) const {
+  __device__ __forceinline__ void get(int c, bool whole, float (*wk)[VEC], float* bk) const {   // c: the thread's first channel, from c0; whole: a multiple of VEC
+    if (whole) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) mix_load<float, VEC>(&w[k][lane * VEC], wk[k]);
-    mix_load<float, VEC>(&b[lane * VEC], bk);
+      for (int k = 0; k < K; ++k) mix_load<float, VEC>(&w[k][c], wk[k]);
+      mix_load<float, VEC>(&b[c], bk);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) wk[k][i] = w[k][c + i];
+        bk[i] = b[c + i];
+      }
+    }
   }
 };
+
+// first channel of group cg: the last group of a width that is no multiple of VEC moves back and shares channels with the one before it (both compute and
+// write the same values)
+template <int VEC> __device__ __forceinline__ int channel_of(int cg, int D) { return cg * VEC + VEC <= D ? cg * VEC : D - VEC; }
 
 template <int VEC, int K> __device__ __forceinline__ void load_weights(const float* w, const float* bias, int d, float (*wk)[VEC], float* bk) {
 #pragma unroll
@@ -53,7 +66,7 @@ template <typename T, int VEC, int K, int M> __device__ __forceinline__ void row
   if (r0 >= K - 1 && r0 - (K - 1) + M <= n) {
     const T* p = x + (int64_t)(r0 - (K - 1)) * sl;
 #pragma unroll
-    for (int i = 0; i < M; ++i) mix_load<T, VEC>(p + i * sl, v[i]);
+    for (int i = 0; i < M; ++i) mix_gload<T, VEC>(p + i * sl, v[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < M; ++i) full_row<T, VEC, K>(x, sl, state, D, r0 + i, n, v[i]);
@@ -66,17 +79,17 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   const int cgb = blk % s.ncgb;
   blk /= s.ncgb;
   const int chb = blk % s.nchb, b = blk / s.nchb, D = s.D, cx = (int)threadIdx.x % s.cx;
-  const int c0 = cgb * s.cx * VEC, nc = D - c0 < s.cx * VEC ? D - c0 : s.cx * VEC;
+  const int c0 = channel_of<VEC>(cgb * s.cx, D), nc = D - c0 < s.cx * VEC ? D - c0 : s.cx * VEC;
   ws.stage(a.w, a.bias, c0, nc);
   const int cg = cgb * s.cx + cx, ch = (chb * s.ty + (int)threadIdx.x / s.cx) * s.runs;   // first run of the thread's
   const int n = mix_length(a.lengths, b, s.L);
   if (cg >= s.ncg || (ch * kRun >= s.L && ch > 0)) return;
-  const int d = cg * VEC;
+  const int d = channel_of<VEC>(cg, D);
   const T* x = (const T*)a.x + b * a.sx_b + d;
   const T* state = a.state ? (const T*)a.state + (int64_t)b * (K - 1) * D + d : nullptr;
   T* y = (T*)a.y + (int64_t)b * s.L * D + d;
   float wk[K][VEC], bk[VEC], win[kRun + K - 1][VEC];
-  ws.get(cx, wk, bk);
+  ws.get(d - c0, D % VEC == 0, wk, bk);
   rows_of<T, VEC, K, K - 1>(x, a.sx_l, state, D, ch * kRun, n, win);
   for (int run = 0; run < s.runs && (ch + run) * kRun < s.L; ++run) {
     const int t0 = (ch + run) * kRun;
@@ -94,7 +107,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
         if (a.act) z *= mix_sigmoid(z);
         o[c] = t < n ? z : 0.0f;
       }
-      mix_store<T, VEC>(y + (int64_t)t * D, o);
+      mix_gstore<T, VEC>(y + (int64_t)t * D, o);
     }
 #pragma unroll
     for (int i = 0; i < K - 1; ++i)
@@ -107,7 +120,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
     for (int j = 0; j < K - 1; ++j) {
       float v[VEC];
       full_row<T, VEC, K>(x, a.sx_l, state, D, n + j, n, v);
-      mix_store<T, VEC>(so + (int64_t)j * D, v);
+      mix_gstore<T, VEC>(so + (int64_t)j * D, v);
     }
   }
 }
@@ -122,7 +135,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   const int cgb = blk % s.ncgb;
   blk /= s.ncgb;
   const int chb = blk % s.nchb, b = blk / s.nchb, D = s.D, cx = (int)threadIdx.x % s.cx, ty = (int)threadIdx.x / s.cx;
-  const int c0 = cgb * s.cx * VEC, nc = D - c0 < s.cx * VEC ? D - c0 : s.cx * VEC;
+  const int c0 = channel_of<VEC>(cgb * s.cx, D), nc = D - c0 < s.cx * VEC ? D - c0 : s.cx * VEC;
   sh.ws.stage(a.w, a.bias, c0, nc);
   const int cg = cgb * s.cx + cx, ch = (chb * s.ty + ty) * s.runs, n = mix_length(a.lengths, b, s.L);
   float gwk[K + 1][VEC];
@@ -131,14 +144,14 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
 #pragma unroll
     for (int c = 0; c < VEC; ++c) gwk[k][c] = 0.0f;
   if (cg < s.ncg && (ch * kRun < s.L || ch == 0)) {
-    const int d = cg * VEC;
+    const int d = channel_of<VEC>(cg, D);
     const T* x = (const T*)a.x + b * a.sx_b + d;
     const T* g = a.gy ? (const T*)a.gy + b * a.sg_b + d : nullptr;
     const T* state = a.state ? (const T*)a.state + (int64_t)b * (K - 1) * D + d : nullptr;
     const T* gs = a.gstate ? (const T*)a.gstate + (int64_t)b * (K - 1) * D + d : nullptr;
     T* gx = (T*)a.gx + (int64_t)b * s.L * D + d;
     float win[kRun + 2 * (K - 1)][VEC], gz[kRun + K - 1][VEC], wk[K][VEC], bk[VEC];
-    sh.ws.get(cx, wk, bk);
+    sh.ws.get(d - c0, D % VEC == 0, wk, bk);
     // gz of position t from its window (rows t .. t + K - 1 of [state; x]); 0 behind the end, where z may be anything
     auto slope = [&](float* v, const float (*row)[VEC], int t) {
       if (!a.act || t >= n) return;
@@ -153,7 +166,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
     };
     auto load_g = [&](float* v, int t) {
       if (g && t < n) {
-        mix_load<T, VEC>(g + (int64_t)t * a.sg_l, v);
+        mix_gload<T, VEC>(g + (int64_t)t * a.sg_l, v);
       } else {
 #pragma unroll
         for (int c = 0; c < VEC; ++c) v[c] = 0.0f;
@@ -178,11 +191,11 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
           for (int c = 0; c < VEC; ++c) o[c] = __builtin_fmaf(wk[r - t][c], gz[t][c], o[c]);
         if (gs && r >= n) {   // a sequence shorter than K-1: the old rows are in the new state
           float v[VEC];
-          mix_load<T, VEC>(gs + (int64_t)(r - n) * D, v);
+          mix_gload<T, VEC>(gs + (int64_t)(r - n) * D, v);
 #pragma unroll
           for (int c = 0; c < VEC; ++c) o[c] += v[c];
         }
-        mix_store<T, VEC>(gi + (int64_t)r * D, o);
+        mix_gstore<T, VEC>(gi + (int64_t)r * D, o);
       }
     }
     for (int run = 0; run < s.runs && (ch + run) * kRun < s.L; ++run) {
@@ -191,7 +204,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
       if (g && t0 + K - 1 + kRun <= n) {
         const T* p = g + (int64_t)(t0 + K - 1) * a.sg_l;
 #pragma unroll
-        for (int i = 0; i < kRun; ++i) mix_load<T, VEC>(p + i * a.sg_l, gz[K - 1 + i]);
+        for (int i = 0; i < kRun; ++i) mix_gload<T, VEC>(p + i * a.sg_l, gz[K - 1 + i]);
       } else {
 #pragma unroll
         for (int i = 0; i < kRun; ++i) load_g(gz[K - 1 + i], t0 + K - 1 + i);
@@ -213,7 +226,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
         const int j = t + K - 1 - n;   // row of the final state that x[t] is
         if (gs && t < n && j >= 0) {
           float v[VEC];
-          mix_load<T, VEC>(gs + (int64_t)j * D, v);
+          mix_gload<T, VEC>(gs + (int64_t)j * D, v);
 #pragma unroll
           for (int c = 0; c < VEC; ++c) o[c] += v[c];
         }
@@ -221,7 +234,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
 #pragma unroll
           for (int c = 0; c < VEC; ++c) o[c] = 0.0f;
         }
-        mix_store<T, VEC>(gx + (int64_t)t * D, o);
+        mix_gstore<T, VEC>(gx + (int64_t)t * D, o);
       }
 #pragma unroll
       for (int i = 0; i < kRun; ++i)   // gz is 0 behind the end
@@ -249,7 +262,7 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
     for (int c = 0; c < VEC; ++c) sh.red[c * 256 + threadIdx.x] = gwk[k][c];
     __syncthreads();
     for (int i = threadIdx.x; i < s.cx * VEC; i += 256) {
-      const int lane = i / VEC, c = i % VEC, dd = (cgb * s.cx + lane) * VEC + c;
+      const int lane = i / VEC, c = i % VEC, dd = channel_of<VEC>(cgb * s.cx + lane, D) + c;
       if (cgb * s.cx + lane < s.ncg) {
         float v = 0.0f;
         for (int q = 0; q < s.ty; ++q) v += sh.red[c * 256 + q * s.cx + lane];
@@ -279,9 +292,9 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
   if (item >= (int64_t)a.B * ncg) return;
   const int b = (int)(item / ncg), d = (int)(item % ncg) * VEC, D = a.D;
   float win[K][VEC], wk[K][VEC], bk[VEC];
-  mix_load<T, VEC>((const T*)a.x + b * a.sx_b + d, win[K - 1]);
+  mix_gload<T, VEC>((const T*)a.x + b * a.sx_b + d, win[K - 1]);
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) mix_load<T, VEC>((const T*)a.state + ((int64_t)b * (K - 1) + k) * D + d, win[k]);
+  for (int k = 0; k < K - 1; ++k) mix_gload<T, VEC>((const T*)a.state + ((int64_t)b * (K - 1) + k) * D + d, win[k]);
   load_weights<VEC, K>(a.w, a.bias, d, wk, bk);
   float o[VEC];
 #pragma unroll
@@ -291,16 +304,16 @@ template <typename T, int VEC, int K> __global__ __launch_bounds__(256) void sho
     for (int k = 0; k < K; ++k) z = __builtin_fmaf(wk[k][c], win[k][c], z);
     o[c] = a.act ? z * mix_sigmoid(z) : z;
   }
-  mix_store<T, VEC>((T*)a.y + (int64_t)b * D + d, o);
+  mix_gstore<T, VEC>((T*)a.y + (int64_t)b * D + d, o);
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) mix_store<T, VEC>((T*)a.state_out + ((int64_t)b * (K - 1) + k) * D + d, win[k + 1]);   // all loads are done: in place is fine
+  for (int k = 0; k < K - 1; ++k) mix_gstore<T, VEC>((T*)a.state_out + ((int64_t)b * (K - 1) + k) * D + d, win[k + 1]);   // all loads are done: in place is fine
 }
 
 Shape shape_of(const w2s_short_conv_args* a, int vec, bool backward) {
   Shape s;
   s.L = a->L;
   s.D = a->D;
-  s.ncg = a->D / vec;
+  s.ncg = (a->D + vec - 1) / vec;
   s.cx = 1;
   while (s.cx < 64 && s.cx < s.ncg) s.cx *= 2;
   s.ty = 256 / s.cx;
@@ -321,17 +334,9 @@ bool valid(const w2s_short_conv_args* a) {
   return a && a->w && a->B >= 0 && a->L >= 0 && a->D >= 1 && a->K >= 1 && a->K <= 8 && a->dtype >= 0 && a->dtype <= 2 && (a->act == 0 || a->act == 1);
 }
 
-// elements a lane: four where every pointer, row and width allows them, one otherwise.  (Eight 16-bit elements, a full 16-byte access, measured 19 % slower
-// forward: twice the window in registers, half the waves; in the backward they do not fit.)
-int vector_of(const w2s_short_conv_args* a) {
-  const int e = esize(a->dtype), v = 4;
-  if (a->D % v) return 1;
-  const void* ps[] = {a->x, a->state, a->y, a->state_out, a->gy, a->gstate, a->gx, a->gstate_in};
-  for (const void* p : ps)
-    if ((uintptr_t)p % (size_t)(v * e)) return 1;
-  if (a->sx_b % v || a->sx_l % v || a->sg_b % v || a->sg_l % v) return 1;
-  return v;
-}
+// elements a thread: four wherever there are four.  (Eight 16-bit elements, a full 16-byte access, measured 19 % slower forward: twice the window in
+// registers, half the waves; in the backward they do not fit.)  The step may write where it reads, so its threads share no channels: one each for other widths.
+int vector_of(const w2s_short_conv_args* a, bool step) { return (step ? a->D % 4 == 0 : a->D >= 4) ? 4 : 1; }
 
 enum { kFwd, kBwd, kStep };
 
@@ -376,7 +381,7 @@ template <typename T, int VEC, bool BWD> int by_taps(const w2s_short_conv_args* 
 
 int dispatch(const w2s_short_conv_args* a, int what, void* stream) {
   hipStream_t st = (hipStream_t)stream;
-  const bool bwd = what == kBwd, wide = vector_of(a) > 1;
+  const bool bwd = what == kBwd, wide = vector_of(a, what == kStep) > 1;
   switch (a->dtype) {
     case W2S_F32:
       if (bwd) return wide ? by_taps<float, 4, true>(a, what, st) : by_taps<float, 1, true>(a, what, st);
@@ -401,7 +406,7 @@ extern "C" int w2s_short_conv_fwd(const w2s_short_conv_args* a, void* stream) {
 
 extern "C" int64_t w2s_short_conv_part(const w2s_short_conv_args* a) {
   if (!valid(a)) return W2S_EINVAL;
-  const Shape s = shape_of(a, vector_of(a), true);
+  const Shape s = shape_of(a, vector_of(a, false), true);
   return (int64_t)a->B * s.nchb * (a->K + 1) * a->D;
 }
 

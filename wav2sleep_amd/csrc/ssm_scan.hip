@@ -144,6 +144,7 @@ template <typename T, int NP, int TILE, int W> struct StageBC {
   int slB, slC;
   unsigned off[PER];
   typedef typename mix_vec<T, 4>::type V;
+  typedef V U __attribute__((aligned(sizeof(T))));   // (at any element: B and C are slices of a projection)
   V v[PER];
   __device__ __forceinline__ void start(const w2s_ssm_args& a, const Where& at, int t, int w, int lane) {
     rowB = (const T*)a.Bm + at.b * a.sB_b + at.g * a.sB_g + t * a.sB_l;
@@ -167,13 +168,13 @@ template <typename T, int NP, int TILE, int W> struct StageBC {
       if (u0 >= 2 * HALF || (isc && !with_c)) continue;
       const T* src = (isc ? rowC : rowB) + (unsigned)forgotten(off[k]);
       if (vbc == 2 && left >= TILE) {
-        v[k] = *reinterpret_cast<const V*>(src);
+        v[k] = *reinterpret_cast<const U*>(src);
       } else {
         const int r = u0 - isc * HALF + lane, n = r % (NP / 4) * 4;
         v[k] = V{};
         if (r / (NP / 4) < left && n < a.N) {
           if (vbc) {
-            v[k] = *reinterpret_cast<const V*>(src);
+            v[k] = *reinterpret_cast<const U*>(src);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -758,20 +759,20 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void ssm_step_k
   for (int j = q * VEC; j < N; j += 4 * VEC) {
     float h[VEC], A[VEC], Bv[VEC], Cv[VEC];
     if (a.h0) {
-      mix_load<float, VEC>(a.h0 + item * N + j, h);
+      mix_gload<float, VEC>(a.h0 + item * N + j, h);
     } else {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) h[i] = 0.0f;
     }
-    mix_load<float, VEC>(a.A + (int64_t)d * N + j, A);
-    mix_load<T, VEC>(Bt + j, Bv);
-    mix_load<T, VEC>(Ct + j, Cv);
+    mix_gload<float, VEC>(a.A + (int64_t)d * N + j, A);
+    mix_gload<T, VEC>(Bt + j, Bv);
+    mix_gload<T, VEC>(Ct + j, Cv);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       h[i] = __builtin_fmaf(__builtin_amdgcn_exp2f(dl * A[i]), h[i], du * Bv[i]);
       y = __builtin_fmaf(Cv[i], h[i], y);
     }
-    mix_store<float, VEC>(a.h_out + item * N + j, h);
+    mix_gstore<float, VEC>(a.h_out + item * N + j, h);
   }
   y = mix_group_sum<4>(y);
   if (q != 0) return;
@@ -782,8 +783,6 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void ssm_step_k
   }
   ((T*)a.y)[item] = (T)y;
 }
-
-int esize(int dtype) { return dtype == W2S_F32 ? 4 : 2; }
 
 // rows within a tile are addressed by 32-bit offsets from the tile's 64-bit base: a position's stride stays below 2^22 elements (128 rows of 4 bytes: 2 GiB)
 bool near(int64_t s) { return s >= 0 && s < (1 << 22); }
@@ -822,9 +821,7 @@ template <int NPL> Plan plan_of(const w2s_ssm_args* a, bool backward, bool* is_w
   p.tps = (p.ntile + p.nseg - 1) / p.nseg;
   if (p.tps > 0) p.nseg = (p.ntile + p.tps - 1) / p.tps;
   if (p.nseg < 1) p.nseg = 1;
-  const int e = esize(a->dtype);
-  p.vbc = a->N % 4 == 0 && mix_aligned(a->Bm, a->sB_b, a->sB_l, 4, e) && a->sB_g % 4 == 0 && mix_aligned(a->Cm, a->sC_b, a->sC_l, 4, e) && a->sC_g % 4 == 0;
-  if (p.vbc && a->N == 4 * NPL) p.vbc = 2;
+  p.vbc = a->N == 4 * NPL ? 2 : a->N % 4 == 0 ? 1 : 0;
   return p;
 }
 
@@ -909,10 +906,7 @@ int scan(const w2s_ssm_args* a, bool backward, void* stream) {
 template <typename T> int step(const w2s_ssm_args* a, hipStream_t st) {
   const int64_t blocks = ((int64_t)a->B * a->D + 63) / 64;
   if (blocks > 0x7fffffff) return W2S_EINVAL;
-  const int bytes = 4 * (int)sizeof(T);   // four states of B and C
-  const bool wide = a->N % 4 == 0 && mix_aligned(a->h0, 0, 0, 4, 4) && mix_aligned(a->h_out, 0, 0, 4, 4) && mix_aligned(a->A, 0, 0, 4, 4) &&
-                    mix_aligned(a->Bm, a->sB_b, a->sB_g, 4, bytes / 4) && mix_aligned(a->Cm, a->sC_b, a->sC_g, 4, bytes / 4);
-  if (wide) ssm_step_kernel<T, 4><<<(unsigned)blocks, 256, 0, st>>>(*a);
+  if (a->N % 4 == 0) ssm_step_kernel<T, 4><<<(unsigned)blocks, 256, 0, st>>>(*a);
   else ssm_step_kernel<T, 1><<<(unsigned)blocks, 256, 0, st>>>(*a);
   W2S_CHECK_LAUNCH();
   return W2S_OK;
