@@ -137,6 +137,28 @@ def test_scan_long_row_gradients():
     check_scan(scan_inputs('f32', 1, 2050, 16, 16, 1, seed=8))
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16'])
+@pytest.mark.parametrize('shape', [(8, 1200, 16, 16, 1), (3, 700, 20, 40, 1), (4, 900, 16, 6, 2), (2, 520, 8, 32, 1)], ids=str)
+def test_scan_ragged_rows_in_segments(dtype, shape):
+    """few workgroups and long sequences, some of which end segments before the last"""
+    check_scan(scan_inputs(dtype, *shape, seed=41, ragged=True, strided=True))
+
+
+def test_scan_far_strides():
+    """positions far apart: of a sequence of one they do not matter, and a gradient that arrives so is copied"""
+    p = scan_inputs('f32', 2, 6, 8, 4, 1, seed=15)
+    flat = torch.zeros(5 * (1 << 22) + 64, device='cuda')
+    far = lambda t: flat.as_strided(t.shape, (t.shape[2], 1 << 22, 1)).copy_(t)   # noqa: E731
+    one = {k: p[k][:, :1] for k in ('dt', 'Bm', 'Cm')}
+    y = W.ssm_scan(far(p['u'][:, :1]), one['dt'], p['A'], one['Bm'], one['Cm'])
+    assert torch.equal(y, W.ssm_scan(p['u'][:, :1], one['dt'], p['A'], one['Bm'], one['Cm']))
+    u = p['u'].clone().requires_grad_(True)
+    y = W.ssm_scan(u, p['dt'], p['A'], p['Bm'], p['Cm'])
+    a, = torch.autograd.grad(y, u, p['gy'], retain_graph=True)
+    b, = torch.autograd.grad(y, u, far(p['gy']))
+    assert torch.equal(a, b)
+
+
 def test_scan_decay_ends():
     """steps so long that the state is forgotten at once, and so short that nothing is"""
     p = scan_inputs('f32', 2, 40, 16, 16, 1, seed=3)
@@ -323,6 +345,32 @@ def test_norm_8bit_marks_a_row_that_is_not_finite():
     x[2, 5] = float('inf')
     q, scale, _ = W.add_rms_norm_8bit(x, w)
     assert torch.isnan(scale[1:3]).all() and torch.isnan(q[1].float()).all() and torch.isfinite(scale[[0, 3]]).all() and torch.isfinite(q[[0, 3]].float()).all()
+
+
+def test_norm_8bit_of_the_smallest_numbers():
+    """a row whose largest value over 448 is below every float: the codes stay numbers, and zeros zeros"""
+    x = torch.tensor([[1.0, 0.0, -1.0, 0.5]], device='cuda').repeat(3, 4)
+    w = torch.full((16,), 1e-43, device='cuda')
+    q, scale, _ = W.add_rms_norm_8bit(x, w)
+    v = q.float()
+    assert (scale > 0).all() and torch.isfinite(v).all() and not v[x == 0].any()
+    want = R.norm(x, w, None)['y']
+    # rstd w and y are multiples of 2^-149, off by half of one each; the scale is exact; half a step of e4m3 is 2^-4 of y
+    assert ((v.double() * scale.double()[:, None] - want).abs() <= 2.0 ** -4 * (want.abs() + 2.0 ** -149) + 2.0 ** -149).all()
+
+
+def test_norm_of_more_rows_than_a_launch_takes():
+    """narrow rows, sixteen a workgroup: 2^28 of them need more than 2^32 threads"""
+    if torch.cuda.mem_get_info()[0] < 8 << 30:
+        pytest.skip('needs 8 GiB')
+    rows = (1 << 28) + 5
+    x = torch.empty(rows, 1, device='cuda', dtype=torch.bfloat16)
+    x[:, 0] = (torch.arange(rows, device='cuda', dtype=torch.int32) % 7 - 3).to(torch.bfloat16)
+    w = torch.full((1,), 2.0, device='cuda')
+    y, _ = W.add_rms_norm(x, w, eps=0.0)
+    assert torch.isnan(y[3]) and torch.equal(y[x != 0], (2 * torch.sign(x))[x != 0])   # x / |x| w, and a zero has no direction
+    q, scale, _ = W.add_rms_norm_8bit(x, w)
+    assert torch.equal(torch.sign(q.view(torch.int8).float()) < 0, x < 0) and (scale[x[:, 0] != 0] > 0).all()
 
 
 # ------------------------------------------------------------------------------------------------------------------ edges that all share
@@ -519,6 +567,33 @@ def test_side_stream_and_two_calls_at_once():
             b1 = call(q)
         torch.cuda.synchronize()
         assert torch.equal(a, a1) and torch.equal(b, b1)
+
+
+def test_steps_in_inference_mode():
+    p = scan_inputs('bf16', 3, 4, 16, 16, 1, seed=20)
+    w = rnd(1, 16, 4)
+    calls = lambda: (W.short_conv_step(p['u'][:, 0], torch.zeros(3, 3, 16, device='cuda', dtype=torch.bfloat16), w),   # noqa: E731
+                     W.ssm_step(p['u'][:, 0], p['dt'][:, 0], p['A'], p['Bm'][:, 0], p['Cm'][:, 0], torch.zeros(3, 16, 16, device='cuda')),
+                     W.ssm_scan(p['u'], p['dt'], p['A'], p['Bm'], p['Cm']), W.short_conv(p['u'], w), W.add_rms_norm(p['u'], w[:, 0], p['z'])[1])
+    want = calls()
+    with torch.inference_mode():
+        got = calls()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_refusals_of_sizes():
+    f = dict(device='cuda')
+    big = torch.zeros(1, 1, 8, **f).expand(1, (1 << 30) + 1, 8)   # (no memory behind it)
+    w = rnd(1, 8, 4)
+    with pytest.raises(ValueError):
+        W.short_conv(big, w)
+    bc = torch.zeros(1, 1, 4, **f).expand(1, (1 << 30) + 1, 4)
+    with pytest.raises(ValueError):
+        W.ssm_scan(big, big, -w, bc, bc)
+    rows = torch.zeros(1, 8, **f).expand(1 << 31, 8)
+    for op in (W.add_rms_norm, W.add_rms_norm_8bit):
+        with pytest.raises(ValueError):
+            op(rows, w[:, 0].contiguous())
 
 
 def test_graphs_replay_forward_and_steps():

@@ -71,7 +71,9 @@ __device__ __forceinline__ float to_fp8_range(float y, float scale) {
   return q != q ? q : fminf(fmaxf(q, -kFp8Max), kFp8Max);
 }
 
-__device__ __forceinline__ float fp8_scale(float top) { return top > 0.0f ? top / kFp8Max : (top == top ? 1.0f : top); }
+__device__ __forceinline__ float fp8_scale(float top) {   // (never 0: 0 / 0 would make the zeros of such a row NaN)
+  return top > 0.0f ? fmaxf(top / kFp8Max, __builtin_bit_cast(float, 1u)) : (top == top ? 1.0f : top);
+}
 
 template <typename T, typename RT, bool FP8, int VEC, int G, int NV> __global__ __launch_bounds__(256) void add_norm_fwd_kernel(w2s_add_norm_args a) {
   __shared__ float red[4];
@@ -303,8 +305,26 @@ __global__ __launch_bounds__(1024) void add_norm_reduce_kernel(const float* part
 int esize(int dtype) { return dtype == W2S_F32 ? 4 : 2; }
 
 bool valid(const w2s_add_norm_args* a) {
-  return a && a->w && a->rows >= 0 && a->rows <= 0x7fffffff && a->C >= 1 && a->dtype >= 0 && a->dtype <= 2 &&
+  return a && a->w && a->rows >= 0 && a->rows <= 0x7fffffff && a->C >= 1 && a->C <= (1 << 30) && a->dtype >= 0 && a->dtype <= 2 &&
          (a->rdtype == a->dtype || a->rdtype == W2S_F32);
+}
+
+constexpr int64_t kMaxBlocks = 0xffffffffLL / 256;   // a launch has fewer than 2^32 threads
+
+// rows r0 .. r0 + n - 1 of a forward call
+w2s_add_norm_args rows_from(const w2s_add_norm_args* a, int64_t r0, int64_t n) {
+  w2s_add_norm_args s = *a;
+  const int e = esize(a->dtype), er = esize(a->rdtype);
+  s.x = (const char*)a->x + r0 * a->ldx * e;
+  s.y = (char*)a->y + r0 * a->C * (a->fp8 ? 1 : e);
+  if (a->res) {
+    s.res = (const char*)a->res + r0 * a->ldres * er;
+    s.r = (char*)a->r + r0 * a->C * er;
+  }
+  if (a->scale) s.scale = a->scale + r0;
+  if (a->rstd) s.rstd = a->rstd + r0;
+  s.rows = n;
+  return s;
 }
 
 // workgroups of the backward: enough for 8 waves a SIMD quad on every CU, at most one per row group
@@ -314,13 +334,17 @@ int bwd_blocks(const w2s_add_norm_args* a) {
 }
 
 template <typename T, typename RT, int VEC, int G, int NV> int go(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
-  const int64_t groups = (a->rows + 256 / G - 1) / (256 / G);
+  constexpr int RPB = 256 / G;
   if (bwd) {
     if constexpr (NV <= 4) add_norm_bwd_kernel<T, RT, VEC, G, NV><<<bwd_blocks(a), 256, 0, st>>>(*a);
-  } else if (a->fp8) {
-    add_norm_fwd_kernel<T, RT, true, VEC, G, NV><<<(unsigned)groups, 256, 0, st>>>(*a);
-  } else {
-    add_norm_fwd_kernel<T, RT, false, VEC, G, NV><<<(unsigned)groups, 256, 0, st>>>(*a);
+    return W2S_OK;
+  }
+  for (int64_t r0 = 0; r0 < a->rows; r0 += kMaxBlocks * RPB) {
+    const int64_t n = a->rows - r0 < kMaxBlocks * RPB ? a->rows - r0 : kMaxBlocks * RPB;
+    const w2s_add_norm_args s = rows_from(a, r0, n);
+    const unsigned blocks = (unsigned)((n + RPB - 1) / RPB);
+    if (a->fp8) add_norm_fwd_kernel<T, RT, true, VEC, G, NV><<<blocks, 256, 0, st>>>(s);
+    else add_norm_fwd_kernel<T, RT, false, VEC, G, NV><<<blocks, 256, 0, st>>>(s);
   }
   return W2S_OK;
 }
@@ -336,23 +360,22 @@ template <typename T, typename RT> int by_width(const w2s_add_norm_args* a, bool
   if (units <= 512) return go<T, RT, V, 256, 2>(a, bwd, st);
   if (units <= 1024) return go<T, RT, V, 256, 4>(a, bwd, st);
   if (units <= 2048 && !bwd) return go<T, RT, V, 256, 8>(a, bwd, st);   // (the backward keeps four such rows: it would spill)
-  if (bwd) {
-    add_norm_bwd_loop_kernel<T, RT><<<bwd_blocks(a), 256, 0, st>>>(*a);
-  } else if (a->fp8) {
-    add_norm_fwd_loop_kernel<T, RT, true><<<(unsigned)a->rows, 256, 0, st>>>(*a);
-  } else {
-    add_norm_fwd_loop_kernel<T, RT, false><<<(unsigned)a->rows, 256, 0, st>>>(*a);
-  }
+  if (!bwd && a->rows > kMaxBlocks) return W2S_EINVAL;   // (more than 2^37 elements)
+  if (bwd) add_norm_bwd_loop_kernel<T, RT><<<bwd_blocks(a), 256, 0, st>>>(*a);
+  else if (a->fp8) add_norm_fwd_loop_kernel<T, RT, true><<<(unsigned)a->rows, 256, 0, st>>>(*a);
+  else add_norm_fwd_loop_kernel<T, RT, false><<<(unsigned)a->rows, 256, 0, st>>>(*a);
   return W2S_OK;
 }
 
 int dispatch(const w2s_add_norm_args* a, bool bwd, hipStream_t st) {
   const bool wide_r = a->rdtype != a->dtype;
+  int rc = W2S_EINVAL;
   switch (a->dtype) {
-    case W2S_F32: by_width<float, float>(a, bwd, st); break;
-    case W2S_BF16: wide_r ? by_width<bf16_t, float>(a, bwd, st) : by_width<bf16_t, bf16_t>(a, bwd, st); break;
-    case W2S_F16: wide_r ? by_width<half_t, float>(a, bwd, st) : by_width<half_t, half_t>(a, bwd, st); break;
+    case W2S_F32: rc = by_width<float, float>(a, bwd, st); break;
+    case W2S_BF16: rc = wide_r ? by_width<bf16_t, float>(a, bwd, st) : by_width<bf16_t, bf16_t>(a, bwd, st); break;
+    case W2S_F16: rc = wide_r ? by_width<half_t, float>(a, bwd, st) : by_width<half_t, half_t>(a, bwd, st); break;
   }
+  if (rc != W2S_OK) return rc;
   if (bwd && a->gw) add_norm_reduce_kernel<<<(a->C + 15) / 16, 1024, 0, st>>>(a->part, bwd_blocks(a), a->C, a->gw);
   W2S_CHECK_LAUNCH();
   return W2S_OK;

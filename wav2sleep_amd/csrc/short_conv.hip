@@ -330,8 +330,10 @@ Shape shape_of(const w2s_short_conv_args* a, int vec, bool backward) {
 
 int esize(int dtype) { return dtype == W2S_F32 ? 4 : 2; }
 
+constexpr int64_t kMaxBlocks = 0xffffffffLL / 256;   // a launch has fewer than 2^32 threads
+
 bool valid(const w2s_short_conv_args* a) {
-  return a && a->w && a->B >= 0 && a->L >= 0 && a->D >= 1 && a->K >= 1 && a->K <= 8 && a->dtype >= 0 && a->dtype <= 2 && (a->act == 0 || a->act == 1);
+  return a && a->w && a->B >= 0 && a->L >= 0 && a->L <= (1 << 30) && a->D >= 1 && a->D <= (1 << 30) && a->K >= 1 && a->K <= 8 && a->dtype >= 0 && a->dtype <= 2 && (a->act == 0 || a->act == 1);
 }
 
 // elements a thread: four wherever there are four.  (Eight 16-bit elements, a full 16-byte access, measured 19 % slower forward: twice the window in
@@ -344,7 +346,7 @@ template <typename T, int VEC, int K, bool BWD> int launch(const w2s_short_conv_
   if constexpr (BWD) {
     const Shape s = shape_of(a, VEC, true);
     const int64_t blocks = (int64_t)a->B * s.nchb * s.ncgb;
-    if (blocks > 0x7fffffff) return W2S_EINVAL;
+    if (blocks > kMaxBlocks) return W2S_EINVAL;
     short_conv_bwd_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, s);
     if (a->part) {
       const int64_t C = (int64_t)(K + 1) * a->D;
@@ -353,12 +355,12 @@ template <typename T, int VEC, int K, bool BWD> int launch(const w2s_short_conv_
   } else if (what == kStep) {
     const int ncg = a->D / VEC;
     const int64_t blocks = ((int64_t)a->B * ncg + 255) / 256;
-    if (blocks > 0x7fffffff) return W2S_EINVAL;
+    if (blocks > kMaxBlocks) return W2S_EINVAL;
     short_conv_step_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, ncg);
   } else {
     const Shape s = shape_of(a, VEC, false);
     const int64_t blocks = (int64_t)a->B * s.nchb * s.ncgb;
-    if (blocks > 0x7fffffff) return W2S_EINVAL;
+    if (blocks > kMaxBlocks) return W2S_EINVAL;
     short_conv_fwd_kernel<T, VEC, K><<<(unsigned)blocks, 256, 0, st>>>(*a, s);
   }
   W2S_CHECK_LAUNCH();

@@ -788,8 +788,10 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void ssm_step_k
 bool near(int64_t s) { return s >= 0 && s < (1 << 22); }
 
 bool valid(const w2s_ssm_args* a) {
-  return a && near(a->su_l) && near(a->sdt_l) && near(a->sz_l) && near(a->sB_l) && near(a->sC_l) && near(a->sg_l) && a->D < (1 << 22) && a->A && a->B >= 0 && a->L >= 0 && a->D >= 1 && a->N >= 1 && a->N <= 64 && a->G >= 1 && a->D % a->G == 0 && a->dtype >= 0 && a->dtype <= 2;
+  return a && near(a->su_l) && near(a->sdt_l) && near(a->sz_l) && near(a->sB_l) && near(a->sC_l) && near(a->sg_l) && near(a->D) && a->A && a->B >= 0 && a->L >= 0 &&
+         a->L <= (1 << 30) && a->D >= 1 && a->N >= 1 && a->N <= 64 && a->G >= 1 && a->D % a->G == 0 && a->dtype >= 0 && a->dtype <= 2;
 }
+bool launches(int64_t blocks, int threads) { return blocks * threads <= 0xffffffffLL; }   // a launch has fewer than 2^32 threads
 
 int npl_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 // Segments a sequence is cut into.  Cutting costs a second walk for the end states (half of a whole one), so it pays only where the workgroups of whole
@@ -844,7 +846,7 @@ template <typename T, int NPL, bool GATE> int scan_fwd(const w2s_ssm_args* a, hi
   bool w;
   Plan p = plan_of<NPL>(a, false, &w);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
-  if (blocks > 0x7fffffff) return W2S_EINVAL;
+  if (!launches(blocks, 1024)) return W2S_EINVAL;
   if (p.nseg > 1) {
     if (!a->ws) return W2S_EINVAL;
     p.segh = (float*)a->ws;
@@ -863,7 +865,7 @@ template <typename T, int NPL, bool GATE> int scan_bwd(const w2s_ssm_args* a, hi
   Plan p = plan_of<NPL>(a, true, &w);
   const int64_t blocks = (int64_t)a->B * a->G * p.ncb * p.nseg;
   const int64_t rows = (int64_t)a->B * a->L * a->G, nbc = (rows * (2 * NPL) + 255) / 256, na = ((int64_t)a->D * (a->N + 2) + 15) / 16;
-  if (blocks > 0x7fffffff || nbc > 0x7fffffff || na > 0x7fffffff) return W2S_EINVAL;
+  if (!launches(blocks, 512) || !launches(nbc, 256) || !launches(na, 1024)) return W2S_EINVAL;
   p.part_bc = (float*)a->ws;
   p.part_a = p.part_bc + bc_floats(a, p, 4 * NPL);
   p.segh = p.part_a + a_floats(a, p);
@@ -905,7 +907,7 @@ int scan(const w2s_ssm_args* a, bool backward, void* stream) {
 
 template <typename T> int step(const w2s_ssm_args* a, hipStream_t st) {
   const int64_t blocks = ((int64_t)a->B * a->D + 63) / 64;
-  if (blocks > 0x7fffffff) return W2S_EINVAL;
+  if (!launches(blocks, 256)) return W2S_EINVAL;
   if (a->N % 4 == 0) ssm_step_kernel<T, 4><<<(unsigned)blocks, 256, 0, st>>>(*a);
   else ssm_step_kernel<T, 1><<<(unsigned)blocks, 256, 0, st>>>(*a);
   W2S_CHECK_LAUNCH();

@@ -65,9 +65,20 @@ bool is(const Tensor& t, const Tensor& ref, at::ScalarType type, at::IntArrayRef
   return t.defined() && t.scalar_type() == type && t.device() == ref.device() && t.sizes() == shape && t.layout() == at::kStrided;
 }
 bool is(const Opt& t, const Tensor& ref, at::ScalarType type, at::IntArrayRef shape) { return !t || is(*t, ref, type, shape); }
-bool io(const Tensor& t, int64_t dim) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && code(t) >= 0 && t.dim() == dim; }
+bool sized(const Tensor& t) {   // every size within 2^30: the descriptors hold 32-bit sizes, the kernels' positions run a tile past them
+  for (const int64_t n : t.sizes())
+    if (n > (1 << 30)) return false;
+  return true;
+}
+bool io(const Tensor& t, int64_t dim) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && code(t) >= 0 && t.dim() == dim && sized(t); }
 
 Tensor rows_of(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }   // contiguous last dimension
+// ... and positions less than 2^22 elements apart, as a scan's kernels want them (32-bit offsets inside a tile); a gradient's layout is not the caller's choice
+Tensor near_rows(const Tensor& t) {
+  const Tensor r = rows_of(t);
+  return r.size(1) <= 1 || r.stride(1) < (1 << 22) ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+int64_t position_stride(const Tensor& t) { return t.defined() && t.size(1) > 1 ? t.stride(1) : 0; }
 Tensor plain(const Opt& t) { return t ? t->contiguous() : Tensor(); }
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor like_if(const Tensor& t) { return t.defined() ? like(t) : Tensor(); }
@@ -218,8 +229,8 @@ py::object short_conv_step(const Tensor& x, const Tensor& state, const Tensor& w
   auto a = conv_args(xr, wc, bc, act, state, Tensor());
   a.y = ptr(y);
   a.state_out = ptr(out);
-  done(entry.conv_step(&a, stream(x)), "w2s_short_conv_step");
   out.unsafeGetTensorImpl()->bump_version();
+  done(entry.conv_step(&a, stream(x)), "w2s_short_conv_step");
   return py::cast(y);
 }
 
@@ -247,11 +258,11 @@ w2s_ssm_args ssm_args(const Ssm& s, int64_t softplus) {
   a.sB_b = s.B.stride(0);
   a.sC_b = s.C.stride(0);
   if (!step) {
-    a.su_l = s.u.stride(1);
-    a.sdt_l = s.dt.stride(1);
-    a.sz_l = s.z.defined() ? s.z.stride(1) : 0;
-    a.sB_l = s.B.stride(1);
-    a.sC_l = s.C.stride(1);
+    a.su_l = position_stride(s.u);
+    a.sdt_l = position_stride(s.dt);
+    a.sz_l = position_stride(s.z);
+    a.sB_l = position_stride(s.B);
+    a.sC_l = position_stride(s.C);
   }
   a.sB_g = s.B.stride(-2);
   a.sC_g = s.C.stride(-2);
@@ -311,11 +322,11 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
       const at::AutoGradMode off(false);
       const c10::DeviceGuard guard(s.u.device());
       auto a = ssm_args(s, k >> 16);
-      Tensor gy = g[0].defined() ? rows_of(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+      Tensor gy = g[0].defined() ? near_rows(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
       a.gy = ptr(gy);
       if (gy.defined()) {
         a.sg_b = gy.stride(0);
-        a.sg_l = gy.stride(1);
+        a.sg_l = position_stride(gy);
       }
       a.gh = ptr<float>(gl);
       a.ckpt = ptr<float>(v[10]);
@@ -358,6 +369,8 @@ bool ssm_ok(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor& B, Tenso
 py::object ssm_scan(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B, Tensor C, const Opt& D, const Opt& z, const Opt& bias, bool softplus, const Opt& state,
                     const Opt& lengths, bool want_state) {
   if (!ssm_ok(u, dt, A, B, C, D, z, bias, state, 3) || !is(lengths, u, at::kInt, {u.size(0)})) return py::none();
+  for (const Opt& t : {Opt(u), Opt(dt), Opt(B), Opt(C), z})
+    if (t && position_stride(*t) >= (1 << 22)) return py::none();
   Tensor y, last;
   {
     const py::gil_scoped_release free;
@@ -385,8 +398,8 @@ py::object ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B
   auto a = ssm_args(s, softplus);
   a.y = ptr(y);
   a.h_out = ptr<float>(out);
-  done(entry.ssm_step(&a, stream(u)), "w2s_ssm_step");
   out.unsafeGetTensorImpl()->bump_version();
+  done(entry.ssm_step(&a, stream(u)), "w2s_ssm_step");
   return py::cast(y);
 }
 
@@ -488,7 +501,8 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 };
 
 bool norm_ok(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
-  if (!x.defined() || !x.is_cuda() || code(x) < 0 || x.layout() != at::kStrided || x.dim() < 1 || x.size(-1) < 1 || !(eps >= 0.0)) return false;
+  if (!x.defined() || !x.is_cuda() || code(x) < 0 || x.layout() != at::kStrided || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > (1 << 30) || x.numel() / x.size(-1) > 0x7fffffff || !(eps >= 0.0))
+    return false;
   return is(w, x, at::kFloat, {x.size(-1)}) && (!res || is(*res, x, x.scalar_type(), x.sizes()) || is(*res, x, at::kFloat, x.sizes()));
 }
 

@@ -8,7 +8,8 @@
 
 They are what `SequenceSSM` runs on; the reference mixes epochs with dilated convolutions only (models/wav2sleep.py:349-390).  The first three are
 differentiable (first order; a second one raises) in every floating argument.  Activations are fp32, bf16 or fp16, all of one type in a call, channels last, with any
-strides in front of a contiguous channel dimension (a tensor with another channel stride is copied first); results are contiguous.  Parameters and the
+strides in front of a contiguous channel dimension (a tensor with another channel stride is copied first; the scan's positions lie less than 2^22 elements
+apart); results are contiguous.  Sizes go up to 2^30 and a launch has fewer than 2^32 threads; a call beyond that raises.  Parameters and the
 scan's states are fp32.  Arithmetic is fp32; a 16-bit result is rounded once.  Everything runs on the current stream of the tensors' device,
 allocates from torch's allocator, never synchronises, and records into a hipGraph.  CPU tensors raise (lib.W2SError): there is no CPU path.
 
@@ -35,6 +36,11 @@ def _ops():
 
 
 # ------------------------------------------------------------------------------------------------------------------ what is wrong with a refused call
+def _sizes(name, t):
+    if any(n > 1 << 30 for n in t.shape):
+        raise ValueError(f'{name}: sizes up to 2^30 expected, got {tuple(t.shape)}')
+
+
 def _io(name, t):
     if not isinstance(t, Tensor):
         raise TypeError(f'{name}: a tensor is wanted, got {type(t).__name__}')
@@ -84,6 +90,7 @@ def _refused(what):
 
 def _conv_check(x, weight, bias, activation):
     _io('x', x)
+    _sizes('x', x)
     if activation not in _ACT:
         raise ValueError(f'{activation=} is unsupported (one of {list(_ACT)})')
     D = x.shape[-1]
@@ -100,6 +107,7 @@ def _ssm_check(u, dt, A, B, C, D, z, dt_bias, state, lengths, nrows):
     _io('u', u)
     if u.dim() != nrows + 1:
         raise ValueError(f'u: {nrows + 1} dimensions expected, got {tuple(u.shape)}')
+    _sizes('u', u)
     rows, Dc = tuple(u.shape[:-1]), u.shape[-1]
     if dt is None or B is None or C is None or A is None:
         raise TypeError('dt, A, B and C: tensors are wanted')
@@ -125,6 +133,8 @@ def _norm_check(x, weight, residual, eps):
     _io('x', x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f'x: [..., C] expected, got {tuple(x.shape)}')
+    if x.shape[-1] > 1 << 30 or x.numel() // x.shape[-1] >= 1 << 31:
+        raise ValueError(f'x: fewer than 2^31 rows of up to 2^30 columns expected, got {tuple(x.shape)}')
     _like('weight', weight, x, (x.shape[-1],), _F32)
     if weight is None:
         raise TypeError('weight: a tensor is wanted')
@@ -180,10 +190,14 @@ def ssm_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor |
         y[b, t, d]    = (sum_n C[b, t, g, n] h[b, t, d, n] + D[d] u[b, t, d]) * silu(z[b, t, d])
 
     u, dt, z [B, L, D]; A [D, N], N <= 64 (negative for a stable scan); B, C [B, L, N] or [B, L, G, N]: channel d belongs to group d // (D / G);
-    D, dt_bias [D].  state [B, D, N]: h in front of position 0 (None: zeros).  return_state: also h at the end, the `state` of a call that goes on."""
+    D, dt_bias [D].  Positions are walked in pieces side by side, each carried on by exp(A * its sum of delta): where that product leaves fp32's range (A * delta
+    far above 0, a scan that grows) the result is not defined.  state [B, D, N]: h in front of position 0 (None: zeros).  return_state: also h at the end, the `state` of a call that goes on."""
     out = _ops().ssm_scan(u, dt, A, B, C, D, z, dt_bias, dt_softplus, state, lengths, return_state)
     if out is None:
         _ssm_check(u, dt, A, B, C, D, z, dt_bias, state, lengths, 2)
+        for name, t in (('u', u), ('dt', dt), ('B', B), ('C', C), ('z', z)):
+            if t is not None and t.shape[1] > 1 and t.stride(1) >= 1 << 22:
+                raise lib.W2SError(f'{name}: positions lie {t.stride(1)} elements apart, 2^22 or more: pass a contiguous copy')
         _refused('ssm_scan')
     return out
 
