@@ -33,3 +33,13 @@ def test_refusals():
         m.step(torch.zeros(1, 32), m.init_state(1))
     with pytest.raises(ValueError):
         m.step(torch.zeros(1, 64), [])
+
+
+def test_refusals_of_a_prompt():
+    m = W.SequenceSSM(64, num_layers=1)
+    with pytest.raises(ValueError):
+        m.prompt(torch.zeros(1, 0, 64))
+    with pytest.raises(ValueError):
+        m.prompt(torch.zeros(1, 3, 64), state=[])
+    with pytest.raises(W.lib.W2SError):
+        m.prompt(torch.zeros(1, 3, 64))

@@ -61,6 +61,53 @@ def test_features_and_steps(shape):
         assert float((y - want[:, t]).abs().max()) <= 1e-3 * size, t
 
 
+def test_prompts_of_unequal_nights_then_steps():
+    """nights of unequal length in one call, in one piece and in two, go on one epoch at a time"""
+    m = mixer().eval()
+    B, S, more = 3, 41, 5
+    x = torch.randn(B, S + more, 64, device='cuda')
+    want = reference(m, x)[0].detach()
+    size = float(want.abs().max())
+    n = torch.tensor([41, 7, 20], device='cuda', dtype=torch.int32)
+    y, state = m.prompt(x[:, :S], lengths=n)
+    first = torch.clamp(n, max=9)
+    y1, st = m.prompt(x[:, :9], lengths=first)
+    late = torch.zeros(B, S, 64, device='cuda')   # the rest of each night, from its 10th epoch on
+    for b in range(B):
+        late[b, :S - int(first[b])] = x[b, int(first[b]):S]
+        assert float((y[b, :int(n[b])] - want[b, :int(n[b])]).abs().max()) <= 1e-3 * size
+        assert float((y1[b, :int(first[b])] - want[b, :int(first[b])]).abs().max()) <= 1e-3 * size
+    _, state2 = m.prompt(late, lengths=(n - first).to(torch.int32), state=st)
+    for i in range(more):
+        now = torch.stack([x[b, int(n[b]) + i] for b in range(B)])
+        for s in (state, state2):
+            got = m.step(now, s)
+            for b in range(B):
+                assert float((got[b] - want[b, int(n[b]) + i]).abs().max()) <= 1e-3 * size, (i, b)
+
+
+def test_steps_replay_from_a_graph():
+    m = mixer().eval()
+    x, state = torch.randn(2, 64, device='cuda'), m.init_state(2)
+    with torch.cuda.stream(torch.cuda.Stream()):
+        m.step(x, state)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = m.step(x, state)
+    for pair in state:
+        for t in pair:
+            t.zero_()
+    live = m.init_state(2)
+    for k in range(4):
+        x.copy_(torch.randn(2, 64, device='cuda'))
+        want = m.step(x, live)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), k
+
+
 def test_later_epochs_do_not_reach_earlier_ones():
     m = mixer().eval()
     x = torch.randn(2, 60, 64, device='cuda')

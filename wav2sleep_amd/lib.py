@@ -829,9 +829,9 @@ def _short_conv_args(x, w, bias, act, **kw):
     return ShortConvArgs(x=_p(x), w=_f(w), bias=_f(bias), B=B, L=L, D=D, K=w.shape[1], dtype=_io(x), act=act, sx_b=x.stride(0), sx_l=x.stride(1), **kw)
 
 
-def short_conv_fwd(x, w, bias, y, act=1, state_out=None):
+def short_conv_fwd(x, w, bias, y, act=1):
     """depthwise causal convolution of x [B, L, D] with w [D, K] (+ SiLU: act 1), from zeros"""
-    a = _short_conv_args(x, w, bias, act, y=_p(y), state_out=_p(state_out))
+    a = _short_conv_args(x, w, bias, act, y=_p(y))
     _chk(load().w2s_short_conv_fwd(C.byref(a), _stream()), 'w2s_short_conv_fwd')
 
 
@@ -849,9 +849,9 @@ def _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, **kw):
                    sC_b=Cm.stride(0), sC_l=Cm.stride(1), sC_g=Cm.stride(2), B=B, L=L, D=Dc, N=A.shape[1], G=Bm.shape[2], dtype=_io(u), softplus=1, **kw)
 
 
-def ssm_scan_fwd(u, dt, A, Bm, Cm, D, z, dt_bias, y, keep=False, h_out=None):
+def ssm_scan_fwd(u, dt, A, Bm, Cm, D, z, dt_bias, y, keep=False):
     """selective scan of [B, L, D] from a zero state; keep: returns what ssm_scan_bwd starts from"""
-    a = _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, y=_p(y), h_out=_f(h_out))
+    a = _ssm_scan_args(u, dt, A, Bm, Cm, D, z, dt_bias, y=_p(y))
     ckpt = torch.empty(max(1, load().w2s_ssm_ckpt(C.byref(a))), device=u.device, dtype=torch.float32) if keep else None
     ws = torch.empty(max(1, load().w2s_ssm_ws(C.byref(a), 0)), device=u.device, dtype=torch.uint8)
     a.ckpt, a.ws = _f(ckpt), _p(ws)

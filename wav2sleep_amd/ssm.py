@@ -5,8 +5,8 @@ stream is mixed one epoch at a time: `step` costs the same for the first epoch a
 
     mixer = SequenceSSM(128, num_layers=2)
     model = Wav2Sleep(encoders, epoch_mixer, mixer, num_classes=4)      # trains through SleepModule / GenericTrainStep like any other configuration
-    state = mixer.init_state(batch)                                     # streaming: features of the newest epoch in, mixed features out
-    y = mixer.step(x_BF, state)
+    y, state = mixer.prompt(x_BSF)                                      # streaming: the night so far (or state = mixer.init_state(batch)), ...
+    y = mixer.step(x_BF, state)                                         # ... then features of the newest epoch in, mixed features out
 
 fp32, like the rest of the path around it.  There is no CPU path (lib.W2SError)."""
 from __future__ import annotations
@@ -78,25 +78,63 @@ class SequenceSSM(nn.Module):
         dev = self.norm_weight.device
         return [(torch.zeros(batch, self.kernel_size - 1, self.inner_dim, device=dev), torch.zeros(batch, self.inner_dim, self.state_dim, device=dev)) for _ in self.layers]
 
-    @torch.no_grad()
-    def step(self, x_BF: Tensor, state: list) -> Tensor:
-        """The newest epoch's features [B, F] -> mixed features [B, F]; `state` (init_state, or an earlier step's) moves on in place."""
+    def _mix(self, x: Tensor, state: list, conv, scan) -> Tensor:
+        """rows x [R, F] through the layers; conv(k, u, state) and scan(k, u, dt, A, B, C, z, state) are layer k's operators"""
         from .wav2sleep import _gen
-        if x_BF.dim() != 2 or x_BF.shape[1] != self.feature_dim:
-            raise ValueError(f'[B, {self.feature_dim}] expected, got {tuple(x_BF.shape)}')
-        if len(state) != len(self.layers):
-            raise ValueError(f'the state of {len(self.layers)} layers expected, got {len(state)}')
         gen = _gen(self)
         gen.training = False
-        r, N, rank = self.dt_rank, self.state_dim, self.dt_rank
+        r, N = self.dt_rank, self.state_dim
         with torch.cuda.device(self.norm_weight.device):
-            x, res = x_BF.float().contiguous(), None
-            for layer, (conv_state, h) in zip(self.layers, state):
+            x, res = x.float().contiguous(), None
+            for k, (layer, (conv_state, h)) in enumerate(zip(self.layers, state)):
                 n, res = mixer_ops.add_rms_norm(x, layer.norm_weight, res, self.norm_eps)
-                u = mixer_ops.short_conv_step(gen.linear(n, layer.in_proj.weight, None), conv_state, layer.conv_weight, layer.conv_bias)
+                u = conv(k, gen.linear(n, layer.in_proj.weight, None), conv_state)
                 dbc = gen.linear(u, layer.x_proj.weight, None)
-                dt = gen.linear(dbc[:, :rank].contiguous(), layer.dt_proj.weight, None)
-                y = mixer_ops.ssm_step(u, dt, -torch.exp(layer.A_log), dbc[:, r:r + N], dbc[:, r + N:], h, D=layer.D, z=gen.linear(n, layer.gate_proj.weight, None),
-                                       dt_bias=layer.dt_bias)
+                dt = gen.linear(dbc[:, :r].contiguous(), layer.dt_proj.weight, None)
+                y = scan(k, u, dt, -torch.exp(layer.A_log), dbc[:, r:r + N], dbc[:, r + N:], gen.linear(n, layer.gate_proj.weight, None), h)
                 x = gen.linear(y, layer.out_proj.weight, None)
             return mixer_ops.add_rms_norm(x, self.norm_weight, res, self.norm_eps)[0]
+
+    def _state_check(self, state: list):
+        if len(state) != len(self.layers):
+            raise ValueError(f'the state of {len(self.layers)} layers expected, got {len(state)}')
+
+    @torch.no_grad()
+    def prompt(self, x_BSF: Tensor, lengths: Tensor | None = None, state: list | None = None):
+        """The epochs of a night so far, [B, S, F] -> (mixed features [B, S, F], state behind them for `step` or another `prompt`).  lengths (int32 [B], on the
+        device): how many of the S epochs each sequence has; features behind them are of no meaning.  state: what stands in front (None: nothing)."""
+        if x_BSF.dim() != 3 or x_BSF.shape[2] != self.feature_dim or x_BSF.shape[0] < 1 or x_BSF.shape[1] < 1:
+            raise ValueError(f'[B, S, {self.feature_dim}] with one epoch at least expected, got {tuple(x_BSF.shape)}')
+        B, S, _ = x_BSF.shape
+        state = self.init_state(B) if state is None else state
+        self._state_check(state)
+        behind = [[None, None] for _ in self.layers]
+        seq = lambda t: t.unflatten(0, (B, S))   # noqa: E731
+
+        def conv(k, u, st):
+            p = self.layers[k]
+            y, behind[k][0] = mixer_ops.short_conv(seq(u), p.conv_weight, p.conv_bias, state=st, lengths=lengths, return_state=True)
+            return y.flatten(0, 1)
+
+        def scan(k, u, dt, A, Bm, Cm, z, h):
+            p = self.layers[k]
+            y, behind[k][1] = mixer_ops.ssm_scan(seq(u), seq(dt), A, seq(Bm), seq(Cm), D=p.D, z=seq(z), dt_bias=p.dt_bias, state=h, lengths=lengths, return_state=True)
+            return y.flatten(0, 1)
+        y = self._mix(x_BSF.reshape(B * S, -1), state, conv, scan)
+        return y.view(B, S, -1), [tuple(s) for s in behind]
+
+    @torch.no_grad()
+    def step(self, x_BF: Tensor, state: list) -> Tensor:
+        """The newest epoch's features [B, F] -> mixed features [B, F]; `state` (init_state, or what prompt returned) moves on in place."""
+        if x_BF.dim() != 2 or x_BF.shape[1] != self.feature_dim:
+            raise ValueError(f'[B, {self.feature_dim}] expected, got {tuple(x_BF.shape)}')
+        self._state_check(state)
+
+        def conv(k, u, st):
+            p = self.layers[k]
+            return mixer_ops.short_conv_step(u, st, p.conv_weight, p.conv_bias)
+
+        def scan(k, u, dt, A, Bm, Cm, z, h):
+            p = self.layers[k]
+            return mixer_ops.ssm_step(u, dt, A, Bm, Cm, h, D=p.D, z=z, dt_bias=p.dt_bias)
+        return self._mix(x_BF, state, conv, scan)
