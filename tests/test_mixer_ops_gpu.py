@@ -347,6 +347,30 @@ def test_norm_8bit_marks_a_row_that_is_not_finite():
     assert torch.isnan(scale[1:3]).all() and torch.isnan(q[1].float()).all() and torch.isfinite(scale[[0, 3]]).all() and torch.isfinite(q[[0, 3]].float()).all()
 
 
+@pytest.mark.parametrize('dtype', list(DTYPES))
+@pytest.mark.parametrize('C', [9, 61, 1021, 1999, 4095, 5001, 8191, 12001, 30001])
+def test_norm_odd_widths(dtype, C):
+    """rows that start at every offset of an access, contiguous and as slices of wider rows"""
+    check_norm(dtype, (19,), C, 'same', seed=C)
+    check_norm(dtype, (19,), C, 'f32' if C % 3 else 'same', strided=True, seed=C)
+    x, w, r = rnd(1, 19, C, dtype=DTYPES[dtype]), rnd(2, C), rnd(3, 19, C, dtype=DTYPES[dtype])
+    q, sc, _ = W.add_rms_norm_8bit(x, w, r)
+    assert torch.equal(torch.isfinite(q.float()), torch.ones_like(q, dtype=torch.bool)) and float(q.float().abs().amax(-1).min()) == 448.0
+
+
+@pytest.mark.parametrize('C', [5, 100, 1021, 3000, 8191, 16384, 16390])
+def test_norm_backward_onto_the_gradient_it_adds(C):
+    """the gradient of r may be where the sum goes, also with many rows a workgroup"""
+    from wav2sleep_amd import lib
+    rows = 2100
+    r, w, g, gr = rnd(1, rows, C), rnd(2, C), rnd(3, rows, C), rnd(4, rows, C)
+    rstd = torch.rsqrt(r.pow(2).mean(-1) + 1e-5)
+    one, gw1, gw2 = torch.empty_like(r), torch.empty_like(w), torch.empty_like(w)
+    lib.add_norm_bwd(r, w, rstd, g, gr, one, gw1, 1e-5)
+    lib.add_norm_bwd(r, w, rstd, g, gr, gr, gw2, 1e-5)
+    assert torch.equal(one, gr) and torch.equal(gw1, gw2)
+
+
 def test_norm_8bit_of_the_smallest_numbers():
     """a row whose largest value over 448 is below every float: the codes stay numbers, and zeros zeros"""
     x = torch.tensor([[1.0, 0.0, -1.0, 0.5]], device='cuda').repeat(3, 4)
