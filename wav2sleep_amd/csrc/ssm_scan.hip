@@ -1,10 +1,11 @@
 // Selective state space scan: delta = softplus(dt + bias), h_t[n] = exp(delta A[n]) h_{t-1}[n] + delta u B_t[n], y_t = (sum_n C_t[n] h_t[n] + D u) silu(z),
 // its backward and its form for one position.
 //
-// The recurrence is sequential in t, and B x D channels do not fill 256 CUs (16 nights x 256 channels = 64 waves of one channel a lane).  So a
-// workgroup of 8 waves takes a tile of 8 TT positions of 16 CPL channels and the waves walk their TT positions side by side, which linearity allows:
-//   1. every wave walks its positions from a zero state and keeps the decays a_t = exp(delta_t A) in registers (the exponentials, on the quarter-rate
-//      unit, are the largest single cost and are computed once);
+// The recurrence is sequential in t, and B x D channels do not fill 256 CUs (16 nights x 256 channels = 64 waves of one channel a lane).  So a workgroup
+// takes 16 channels of one group and a tile of W TT positions (W = 16 or 8 waves, TT = 8 or 4 positions each), and the waves walk their positions side by
+// side, which linearity allows:
+//   1. every wave walks its positions from a zero state and keeps the decays a_t = exp(delta_t A) in registers (the exponentials run at a quarter of the
+//      rate, are the largest single cost and are computed once);
 //   2. the waves' end states and products of decays (exp(A sum delta): one more exponential, no product chain) meet in LDS, and each wave folds those
 //      in front of it onto the tile's initial state;
 //   3. every wave walks its positions again from the right state -- two fused steps per state, no exponential -- and emits y.
@@ -12,7 +13,9 @@
 // gate are computed once per quad (the lane of position t mod 4) and broadcast by DPP.  B and C of a tile are staged in LDS in fp32, once per workgroup.
 // A tile's global loads are issued one tile ahead.  Where even that leaves CUs idle (few sequences, few channels) the sequence is cut into
 // segments: a first launch walks them for their end states alone, the second folds the ones in front of its own segment first.
-// Bound: vector issue (about 10 slots per state and position forward, 22 backward, against 4 - 16 bytes per channel and position).
+// Bound: the vector units (counters: 72 % busy forward, 66 - 76 % backward; 13.4 M and 33.1 M wave instructions), not HBM.  Measured, N = 16, gated: 16 nights
+// x 960 x 256 fp32 (65 MB) 38 us forward = 1.7 TB/s, with the backward 149 us (130 MB by the least count, 0.9 TB/s); 4 x 2047 x 1536 bf16 in three groups
+// 124 + 330 us; one row of 16384 x 512 bf16 107 us.  One state a lane and positions one after another, without tiles, took 58 us for a night.
 #include "mix_io.h"
 
 namespace {
@@ -65,10 +68,12 @@ __device__ __forceinline__ float sum_quads_of_row(float v) {   // over the four 
   return v;
 }
 
-// Tile shapes: W waves, TT positions a wave, SIMD waves a SIMD (what the registers have to allow).  WIDE where there is at most one workgroup a CU (and nothing to be gained from cutting sequences): the forward then
-// takes sixteen waves, which hide each other's LDS and barrier waits, and the backward eight with a long walk each.  With more workgroups than CUs, eight
-// waves of at most 128 registers a lane, so that a CU holds two workgroups and the last round of them is short.  From eight states a lane on the registers
-// of a walk leave one.
+// Tile shapes: W waves, TT positions a wave, SIMD waves a SIMD (what the registers have to allow).
+// WIDE where there is at most one workgroup a CU and nothing to gain from cutting sequences: the forward then takes sixteen waves, which hide each other's LDS
+// and barrier waits, and the backward eight with a long walk each (sixteen: 109 us against 100).  With more workgroups than CUs, eight waves of at most 128
+// registers a lane, so that a CU holds two workgroups and the last round of them is short.  fp32, L = 960, D = 256, N = 16, wide / not, forward and with the
+// backward: 256 workgroups 38 / 43 and 141 / 165 us, 288 workgroups 72 / 59 and 262 / 228 us, 512 workgroups 74 / 60 and 284 / 252 us.
+// From eight states a lane on the registers of a walk leave one shape; at 16 states a lane TT = 4 (forward of N = 64, 16 x 960 x 256: 174 us; TT = 8 spills: 276).
 template <int NPL, bool WIDE> struct FwdShape { static constexpr int W = NPL <= 4 && WIDE ? 16 : 8, TT = NPL <= 8 ? 8 : 4, SIMD = NPL <= 4 ? 4 : 2; };
 template <int NPL, bool WIDE> struct BwdShape { static constexpr int W = 8, TT = NPL == 16 || (NPL <= 4 && !WIDE) ? 4 : 8, SIMD = NPL <= 4 && !WIDE ? 4 : 2; };
 
@@ -743,7 +748,8 @@ __global__ __launch_bounds__(1024) void ssm_reduce_a_kernel(w2s_ssm_args a, int 
   else if (a.gbias) a.gbias[d] = v;
 }
 
-// One position.  Four lanes share a channel: with VEC = 4 they read its states as consecutive 16-byte pieces.
+// One position.  Bound by HBM: 8 N bytes of state a channel, read and written.  Four lanes share a channel; with N a multiple of 4 they read its states as
+// consecutive 16-byte pieces (256 x 512 channels, N = 16: 5.7 us against 6.9 one by one; 2048 x 512: 27 us = 5.5 TB/s against 35).
 template <typename T, int VEC> __global__ __launch_bounds__(256) void ssm_step_kernel(w2s_ssm_args a) {
   const int64_t item = (int64_t)blockIdx.x * 64 + (threadIdx.x >> 2);
   const int q = threadIdx.x & 3, N = a.N;
@@ -795,7 +801,9 @@ bool launches(int64_t blocks, int threads) { return blocks * threads <= 0xffffff
 
 int npl_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 // Segments a sequence is cut into.  Cutting costs a second walk for the end states (half of a whole one), so it pays only where the workgroups of whole
-// sequences leave half of the 256 CUs idle or more: then up to two workgroups a CU, of two tiles at least.
+// sequences leave half of the 256 CUs idle or more: then up to two workgroups a CU, of two tiles at least.  fp32, L = 960, D = 256, cut / whole, forward and
+// with the backward: 16 workgroups 20 / 36 and 66 / 134 us, 128 workgroups 33 / 37 and 111 / 139 us, 192 workgroups 45 / 37 and 149 / 140 us; one row of
+// 16384 x 512 bf16 113 / 515 and 352 / 1967 us.
 int segments(int64_t blocks, int ntile) {
   if (blocks <= 0 || blocks > 128 || ntile < 4) return 1;
   int64_t n = 512 / blocks;
