@@ -464,7 +464,8 @@ typedef struct w2s_add_norm_args {
 } w2s_add_norm_args;
 int w2s_add_norm_fwd(const w2s_add_norm_args* a, void* stream);
 int64_t w2s_add_norm_part(const w2s_add_norm_args* a);       /* floats of `part` that w2s_add_norm_bwd needs */
-/* the sum comes from x + res again; x = NULL: from res alone (r saved in fp32).  gx: dtype; gres: rdtype (NULL: not wanted or the same as gx) */
+/* the sum comes from x + res again; x = NULL: from res alone (r saved in fp32).  gx: dtype; gres: rdtype (NULL: not wanted or the same as gx).
+ * Of one type, gr may be gx itself: the gradient is then added to where it is. */
 int w2s_add_norm_bwd(const w2s_add_norm_args* a, void* stream);
 
 const char* w2s_version(void);
