@@ -4,6 +4,7 @@
 // caller then finds out which one and raises.  The kernels' entry points are handed over as addresses (bind), so that the library is loaded once, by lib.py.
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -85,7 +86,14 @@ Tensor like_if(const Tensor& t) { return t.defined() ? like(t) : Tensor(); }
 template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
 bool wants(const Opt& t) { return t && t->requires_grad(); }
 template <typename... Ts> bool graph(const Ts&... t) { return at::GradMode::is_enabled() && (wants(t) || ...); }
-Opt opt(const Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
+// a tangent of forward-mode differentiation: no kernel here carries one on, and a result without it would be a derivative of 0
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool tangent(const Opt& t) { return t && tangent(*t); }
+template <typename... Ts> bool forward_mode(const Ts&... t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && (tangent(t) || ...); }
+void no_forward_mode(const variable_list& g) {   // of gradients that arrive at a node
+  for (const Tensor& t : g)
+    if (forward_mode(t)) throw Failure("this operator's gradient has no forward-mode derivative: a gradient that arrived carries a tangent");
+}
 
 // The gradients are kernels' results: a graph through them (create_graph) has to end in an error, not in a constant
 variable_list first_order(variable_list grads) {
@@ -144,6 +152,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
     return want_state ? variable_list{y, last} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_forward_mode(g);
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &bias = s[2], &state = s[3], &lengths = s[4];
     const int64_t k = ctx->saved_data["k"].toInt();
@@ -195,7 +204,7 @@ bool conv_ok(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& state
 py::object pair_or_one(const Tensor& y, const Tensor& last, bool both) { return both ? py::object(py::make_tuple(y, last)) : py::cast(y); }
 
 py::object short_conv(const Tensor& x, const Tensor& w, const Opt& bias, int64_t act, const Opt& state, const Opt& lengths, bool want_state) {
-  if (!conv_ok(x, w, bias, state, 3) || !is(lengths, x, at::kInt, {x.size(0)})) return py::none();
+  if (!conv_ok(x, w, bias, state, 3) || !is(lengths, x, at::kInt, {x.size(0)}) || forward_mode(x, w, bias, state)) return py::none();
   Tensor y, last;
   {
     const py::gil_scoped_release free;
@@ -221,7 +230,7 @@ bool step_state_ok(const Tensor& state, const Tensor& out) {
 }
 
 py::object short_conv_step(const Tensor& x, const Tensor& state, const Tensor& w, const Opt& bias, int64_t act, const Opt& state_out) {
-  if (!conv_ok(x, w, bias, state, 2) || graph(Opt(x), Opt(state), Opt(w), bias)) return py::none();
+  if (!conv_ok(x, w, bias, state, 2) || graph(Opt(x), Opt(state), Opt(w), bias) || forward_mode(x, state, w, bias, state_out)) return py::none();
   const Tensor& out = state_out ? *state_out : state;
   if (!is(out, x, x.scalar_type(), state.sizes()) || !step_state_ok(state, out)) return py::none();
   const c10::DeviceGuard guard(x.device());
@@ -314,6 +323,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
     return want_state ? variable_list{y, last} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_forward_mode(g);
     const auto v = ctx->get_saved_variables();
     const Ssm s{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9]};
     const int64_t k = ctx->saved_data["k"].toInt();
@@ -368,7 +378,7 @@ bool ssm_ok(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor& B, Tenso
 
 py::object ssm_scan(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B, Tensor C, const Opt& D, const Opt& z, const Opt& bias, bool softplus, const Opt& state,
                     const Opt& lengths, bool want_state) {
-  if (!ssm_ok(u, dt, A, B, C, D, z, bias, state, 3) || !is(lengths, u, at::kInt, {u.size(0)})) return py::none();
+  if (!ssm_ok(u, dt, A, B, C, D, z, bias, state, 3) || !is(lengths, u, at::kInt, {u.size(0)}) || forward_mode(u, dt, A, B, C, D, z, bias, state)) return py::none();
   for (const Opt& t : {Opt(u), Opt(dt), Opt(B), Opt(C), z})
     if (t && position_stride(*t) >= (1 << 22)) return py::none();
   Tensor y, last;
@@ -389,7 +399,9 @@ py::object ssm_scan(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B
 
 py::object ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B, Tensor C, const Tensor& state, const Opt& D, const Opt& z, const Opt& bias, bool softplus,
                     const Opt& state_out) {
-  if (!ssm_ok(u, dt, A, B, C, D, z, bias, state, 2) || graph(Opt(u), Opt(dt), Opt(A), Opt(B), Opt(C), Opt(state), D, z, bias)) return py::none();
+  if (!ssm_ok(u, dt, A, B, C, D, z, bias, state, 2) || graph(Opt(u), Opt(dt), Opt(A), Opt(B), Opt(C), Opt(state), D, z, bias) ||
+      forward_mode(u, dt, A, B, C, state, D, z, bias, state_out))
+    return py::none();
   const Tensor& out = state_out ? *state_out : state;
   if (!is(out, u, at::kFloat, state.sizes()) || !step_state_ok(state, out)) return py::none();
   const c10::DeviceGuard guard(u.device());
@@ -456,6 +468,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
     return res.defined() ? variable_list{y, r} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    no_forward_mode(g);
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &res = s[1], &w = s[2], &rstd = s[3], &first = x.defined() ? x : res;
     const int64_t k = ctx->saved_data["k"].toInt(), C = w.size(0);
@@ -507,7 +520,7 @@ bool norm_ok(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
 }
 
 py::object add_rms_norm(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
-  if (!norm_ok(x, w, res, eps)) return py::none();
+  if (!norm_ok(x, w, res, eps) || forward_mode(x, w, res)) return py::none();
   Tensor y, r, scale, rstd;
   {
     const py::gil_scoped_release free;
@@ -523,7 +536,7 @@ py::object add_rms_norm(const Tensor& x, const Tensor& w, const Opt& res, double
 }
 
 py::object add_rms_norm_8bit(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
-  if (!norm_ok(x, w, res, eps) || graph(Opt(x), Opt(w), res)) return py::none();
+  if (!norm_ok(x, w, res, eps) || graph(Opt(x), Opt(w), res) || forward_mode(x, w, res)) return py::none();
   Tensor y, r, scale, rstd;
   norm_forward(x, w.contiguous(), res ? *res : Tensor(), eps, true, false, y, r, scale, rstd);
   return py::make_tuple(y, scale, res ? r : x);

@@ -7,11 +7,12 @@
     y          = short_conv_step(...) / ssm_step(...)    one position of a stream: the state goes in and comes out
 
 They are what `SequenceSSM` runs on; the reference mixes epochs with dilated convolutions only (models/wav2sleep.py:349-390).  The first three are
-differentiable (first order; a second one raises) in every floating argument.  Activations are fp32, bf16 or fp16, all of one type in a call, channels last, with any
-strides in front of a contiguous channel dimension (a tensor with another channel stride is copied first; the scan's positions lie less than 2^22 elements
-apart); results are contiguous.  Sizes go up to 2^30 and a launch has fewer than 2^32 threads; a call beyond that raises.  Parameters and the
-scan's states are fp32.  Arithmetic is fp32; a 16-bit result is rounded once.  Everything runs on the current stream of the tensors' device,
-allocates from torch's allocator, never synchronises, and records into a hipGraph.  CPU tensors raise (lib.W2SError): there is no CPU path.
+differentiable in every floating argument: in reverse mode, first order (a second one raises), and not in forward mode (an argument or an arriving gradient
+with a tangent raises, in all six).  Activations are fp32, bf16 or fp16, all of one type in a call, channels last, with any strides in front of a contiguous
+channel dimension (a tensor with another channel stride is copied first; the scan's positions lie less than 2^22 elements apart); results are contiguous.
+Sizes go up to 2^30 and a launch has fewer than 2^32 threads; a call beyond that raises.  Parameters and the scan's states are fp32.  Arithmetic is fp32; a
+16-bit result is rounded once.  Everything runs on the current stream of the tensors' device, allocates from torch's allocator, never synchronises, and
+records into a hipGraph.  CPU tensors raise (lib.W2SError): there is no CPU path.
 
 lengths (int32 [B], on the device): sequence b ends in front of position lengths[b], clamped to [0, L].  Inputs at and behind the end are not read,
 results and gradients there are 0, and a returned state is the one at the end (the initial state for a length of 0).
@@ -20,6 +21,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import lib
 
@@ -84,7 +86,13 @@ def _state_check(state, state_out):
         raise lib.W2SError('state_out requires a gradient: a step overwrites it')
 
 
-def _refused(what):
+def no_forward_mode(what, *ts):
+    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise lib.W2SError(f'{what} has no forward-mode derivative: an argument carries a tangent')
+
+
+def _refused(what, *ts):
+    no_forward_mode(what, *ts)
     raise lib.W2SError(f'{what}: arguments refused (dense tensors are wanted)')
 
 
@@ -162,7 +170,7 @@ def short_conv(x: Tensor, weight: Tensor, bias: Tensor | None = None, activation
         _conv_check(x, weight, bias, activation)
         _like('state', state, x, (x.shape[0], weight.shape[1] - 1, x.shape[2]))
         _like('lengths', lengths, x, (x.shape[0],), torch.int32)
-        _refused('short_conv')
+        _refused('short_conv', x, weight, bias, state)
     return out
 
 
@@ -178,7 +186,7 @@ def short_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Tensor | Non
         _conv_check(x, weight, bias, activation)
         _like('state', state, x, (x.shape[0], weight.shape[1] - 1, x.shape[1]))
         _state_check(state, state_out)
-        _refused('short_conv_step')
+        _refused('short_conv_step', x, state, weight, bias, state_out)
     return out
 
 
@@ -198,7 +206,7 @@ def ssm_scan(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, D: Tensor |
         for name, t in (('u', u), ('dt', dt), ('B', B), ('C', C), ('z', z)):
             if t is not None and t.shape[1] > 1 and t.stride(1) >= 1 << 22:
                 raise lib.W2SError(f'{name}: positions lie {t.stride(1)} elements apart, 2^22 or more: pass a contiguous copy')
-        _refused('ssm_scan')
+        _refused('ssm_scan', u, dt, A, B, C, D, z, dt_bias, state)
     return out
 
 
@@ -211,7 +219,7 @@ def ssm_step(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tens
         _no_grad_path('ssm_step', u, dt, A, B, C, state, D, z, dt_bias)
         _ssm_check(u, dt, A, B, C, D, z, dt_bias, state, None, 1)
         _state_check(state, state_out)
-        _refused('ssm_step')
+        _refused('ssm_step', u, dt, A, B, C, state, D, z, dt_bias, state_out)
     return out
 
 
@@ -221,7 +229,7 @@ def add_rms_norm(x: Tensor, weight: Tensor, residual: Tensor | None = None, eps:
     out = _ops().add_rms_norm(x, weight, residual, eps)
     if out is None:
         _norm_check(x, weight, residual, eps)
-        _refused('add_rms_norm')
+        _refused('add_rms_norm', x, weight, residual)
     return out
 
 
@@ -232,5 +240,5 @@ def add_rms_norm_8bit(x: Tensor, weight: Tensor, residual: Tensor | None = None,
     if out is None:
         _norm_check(x, weight, residual, eps)
         _no_grad_path('add_rms_norm_8bit', x, weight, residual)
-        _refused('add_rms_norm_8bit')
+        _refused('add_rms_norm_8bit', x, weight, residual)
     return out

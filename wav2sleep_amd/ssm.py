@@ -70,6 +70,7 @@ class SequenceSSM(nn.Module):
         """[B, S, F] -> [B, S, F] (inference; training goes through Wav2Sleep.forward)."""
         from .wav2sleep import _gen
         gen = _gen(self)
+        mixer_ops.no_forward_mode('SequenceSSM', x_BSF, *self.parameters())
         with torch.cuda.device(self.norm_weight.device):
             return gen.sequence_ssm(self, x_BSF)
 
