@@ -59,3 +59,42 @@ def test_forward_mode_over_a_gradient_is_refused(name):
         with pytest.raises(RuntimeError, match='forward-mode'):
             torch.autograd.grad(y, x, forward_ad.make_dual(gy, gy), retain_graph=True)
     assert torch.isfinite(torch.autograd.grad(y, x, gy)[0]).all()
+
+
+@pytest.mark.parametrize('name', OPERATORS)
+def test_negative_views_and_zeros_without_memory(name):
+    """a real tensor may stand for the negative of what lies in memory (a part of a conjugate), or for zeros that lie nowhere"""
+    run = lambda kw: [t for t in (lambda o: o if isinstance(o, tuple) else (o,))(f(**kw))] + [kw[k] for k in kw if k == 'state_out']   # noqa: E731
+    f, kw = calls()[name]
+    fresh = lambda: {k: v.clone() for k, v in kw.items()}   # noqa: E731
+    for k, v in kw.items():
+        if k == 'state_out' or (k == 'state' and 'state_out' in kw):   # a step's states have to lie in memory
+            for odd in (torch._neg_view(v.clone()), torch._efficientzerotensor(v.shape, device='cuda')):
+                with pytest.raises(W.lib.W2SError):
+                    f(**{**fresh(), k: odd})
+            continue
+        want = run(fresh())
+        for a, b in zip(run({**fresh(), k: torch._neg_view(-v)}), want):
+            assert torch.equal(a.float(), b.float()), k
+        for a, b in zip(run({**fresh(), k: torch._efficientzerotensor(v.shape, device='cuda')}), run({**fresh(), k: torch.zeros_like(v)})):
+            assert torch.equal(a.float(), b.float()), k
+
+
+@pytest.mark.parametrize('name', ['short_conv', 'ssm_scan', 'add_rms_norm'])
+def test_gradients_of_and_through_negative_views(name):
+    f, kw = calls()[name]
+    first = lambda o: o[0] if isinstance(o, tuple) else o   # noqa: E731
+
+    def grads(odd):
+        leaves = {k: v.clone().requires_grad_(True) for k, v in kw.items()}
+        y = first(f(**{k: (torch._neg_view(-v) if odd else v) for k, v in leaves.items()}))
+        gy = rnd(30, *y.shape)
+        return torch.autograd.grad(y, list(leaves.values()), torch._neg_view(-gy) if odd else gy)
+    for k, a, b in zip(kw, grads(True), grads(False)):
+        assert torch.equal(a, b), k
+
+
+def test_a_conjugates_imaginary_part_of_one_channel():
+    c = torch.complex(rnd(1, 2, 6, 1), rnd(2, 2, 6, 1))
+    x, w = c.conj().imag, rnd(3, 1, 4)
+    assert x.is_neg() and torch.equal(W.short_conv(x, w), W.short_conv(x.clone(), w))

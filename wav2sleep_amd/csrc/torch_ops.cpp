@@ -73,14 +73,21 @@ bool sized(const Tensor& t) {   // every size within 2^30: the descriptors hold 
 }
 bool io(const Tensor& t, int64_t dim) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && code(t) >= 0 && t.dim() == dim && sized(t); }
 
-Tensor rows_of(const Tensor& t) { return t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous(); }   // contiguous last dimension
+// A tensor's values may not be what lies at its address: a view that stands for the negative (part of a conjugate), a zero without memory
+bool lies(const Tensor& t) { return !t.is_neg() && !t._is_zerotensor(); }
+Tensor lying(const Tensor& t) { return lies(t) ? t : t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
+Tensor rows_of(const Tensor& t) {   // contiguous last dimension
+  const Tensor r = lying(t);
+  return r.size(-1) <= 1 || r.stride(-1) == 1 ? r : r.contiguous();
+}
 // ... and positions less than 2^22 elements apart, as a scan's kernels want them (32-bit offsets inside a tile); a gradient's layout is not the caller's choice
 Tensor near_rows(const Tensor& t) {
   const Tensor r = rows_of(t);
   return r.size(1) <= 1 || r.stride(1) < (1 << 22) ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 int64_t position_stride(const Tensor& t) { return t.defined() && t.size(1) > 1 ? t.stride(1) : 0; }
-Tensor plain(const Opt& t) { return t ? t->contiguous() : Tensor(); }
+Tensor plain(const Tensor& t) { return lying(t).contiguous(); }
+Tensor plain(const Opt& t) { return t ? plain(*t) : Tensor(); }
 Tensor like(const Tensor& t) { return at::empty(t.sizes(), t.options()); }
 Tensor like_if(const Tensor& t) { return t.defined() ? like(t) : Tensor(); }
 template <typename T = void> T* ptr(const Tensor& t) { return t.defined() ? (T*)t.data_ptr() : nullptr; }
@@ -142,7 +149,7 @@ void conv_forward(w2s_short_conv_args& a, const Tensor& x, bool want_state, Tens
 
 struct ShortConv : torch::autograd::Function<ShortConv> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x_, const Tensor& w_, const Opt& bias_, const Opt& state_, const Opt& lengths_, int64_t act, bool want_state) {
-    const Tensor x = rows_of(x_), w = w_.contiguous(), bias = plain(bias_), state = plain(state_), lengths = plain(lengths_);
+    const Tensor x = rows_of(x_), w = plain(w_), bias = plain(bias_), state = plain(state_), lengths = plain(lengths_);
     auto a = conv_args(x, w, bias, act, state, lengths);
     Tensor y, last;
     conv_forward(a, x, want_state, y, last);
@@ -161,7 +168,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
     {
       const at::AutoGradMode off(false);
       const c10::DeviceGuard guard(x.device());
-      Tensor gy = g[0].defined() ? rows_of(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+      Tensor gy = g[0].defined() ? rows_of(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? plain(g[1]) : Tensor();
       if (need_s) gs = like(state);
       if (x.size(0) == 0 || x.size(1) == 0) {   // no positions: nothing but the state's rows, which pass through
         gx = like(x);
@@ -213,7 +220,7 @@ py::object short_conv(const Tensor& x, const Tensor& w, const Opt& bias, int64_t
       y = out[0];
       if (want_state) last = out[1];
     } else {
-      const Tensor xr = rows_of(x), wc = w.contiguous(), bc = plain(bias), sc = plain(state), lc = plain(lengths);
+      const Tensor xr = rows_of(x), wc = plain(w), bc = plain(bias), sc = plain(state), lc = plain(lengths);
       auto a = conv_args(xr, wc, bc, act, sc, lc);
       conv_forward(a, xr, want_state, y, last);
     }
@@ -223,7 +230,7 @@ py::object short_conv(const Tensor& x, const Tensor& w, const Opt& bias, int64_t
 
 // where a step may leave its state: another tensor than the one it reads only where the two do not overlap
 bool step_state_ok(const Tensor& state, const Tensor& out) {
-  if (!state.is_contiguous() || !out.is_contiguous() || out.requires_grad()) return false;
+  if (!state.is_contiguous() || !out.is_contiguous() || !lies(state) || !lies(out) || out.requires_grad()) return false;
   const char *a = (const char*)state.data_ptr(), *b = (const char*)out.data_ptr();
   const int64_t n = state.numel() * state.element_size();
   return a == b || a + n <= b || b + n <= a;
@@ -234,7 +241,7 @@ py::object short_conv_step(const Tensor& x, const Tensor& state, const Tensor& w
   const Tensor& out = state_out ? *state_out : state;
   if (!is(out, x, x.scalar_type(), state.sizes()) || !step_state_ok(state, out)) return py::none();
   const c10::DeviceGuard guard(x.device());
-  const Tensor xr = rows_of(x), wc = w.contiguous(), bc = plain(bias), y = like(xr);
+  const Tensor xr = rows_of(x), wc = plain(w), bc = plain(bias), y = like(xr);
   auto a = conv_args(xr, wc, bc, act, state, Tensor());
   a.y = ptr(y);
   a.state_out = ptr(out);
@@ -309,7 +316,7 @@ void scan_forward(const Ssm& s, int64_t softplus, bool want_state, bool train, T
 struct SsmScan : torch::autograd::Function<SsmScan> {
   static variable_list forward(AutogradContext* ctx, const Tensor& u, const Tensor& dt, const Tensor& A, const Tensor& B, const Tensor& C, const Opt& D, const Opt& z,
                                const Opt& bias, const Opt& state, const Opt& lengths, int64_t softplus, bool want_state) {
-    const Ssm s{rows_of(u), rows_of(dt), A.contiguous(), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), plain(state), plain(lengths)};
+    const Ssm s{rows_of(u), rows_of(dt), plain(A), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), plain(state), plain(lengths)};
     Tensor y, last, ckpt;
     scan_forward(s, softplus, want_state, true, y, last, ckpt);
     ctx->save_for_backward({s.u, s.dt, s.A, s.B, s.C, s.D, s.z, s.bias, s.state, s.lengths, ckpt});
@@ -332,7 +339,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
       const at::AutoGradMode off(false);
       const c10::DeviceGuard guard(s.u.device());
       auto a = ssm_args(s, k >> 16);
-      Tensor gy = g[0].defined() ? near_rows(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? g[1].contiguous() : Tensor();
+      Tensor gy = g[0].defined() ? near_rows(g[0]) : Tensor(), gl = g.size() > 1 && g[1].defined() ? plain(g[1]) : Tensor();
       a.gy = ptr(gy);
       if (gy.defined()) {
         a.sg_b = gy.stride(0);
@@ -390,7 +397,7 @@ py::object ssm_scan(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B
       if (want_state) last = out[1];
     } else {
       Tensor ckpt;
-      const Ssm s{rows_of(u), rows_of(dt), A.contiguous(), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), plain(state), plain(lengths)};
+      const Ssm s{rows_of(u), rows_of(dt), plain(A), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), plain(state), plain(lengths)};
       scan_forward(s, softplus, want_state, false, y, last, ckpt);
     }
   }
@@ -405,7 +412,7 @@ py::object ssm_step(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor B
   const Tensor& out = state_out ? *state_out : state;
   if (!is(out, u, at::kFloat, state.sizes()) || !step_state_ok(state, out)) return py::none();
   const c10::DeviceGuard guard(u.device());
-  const Ssm s{rows_of(u), rows_of(dt), A.contiguous(), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), state, Tensor()};
+  const Ssm s{rows_of(u), rows_of(dt), plain(A), rows_of(B), rows_of(C), plain(D), z ? rows_of(*z) : Tensor(), plain(bias), state, Tensor()};
   const Tensor y = like(s.u);
   auto a = ssm_args(s, softplus);
   a.y = ptr(y);
@@ -457,7 +464,7 @@ void norm_forward(const Tensor& x, const Tensor& w, const Tensor& res, double ep
 
 struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w_, const Opt& res_, double eps) {
-    const Tensor w = w_.contiguous(), res = res_ ? *res_ : Tensor();
+    const Tensor w = plain(w_), res = res_ ? *res_ : Tensor();
     Tensor y, r, scale, rstd;
     norm_forward(x, w, res, eps, false, true, y, r, scale, rstd);
     // the backward needs the sum as it was normalised: r where that is exact (fp32), else the two addends again
@@ -529,7 +536,7 @@ py::object add_rms_norm(const Tensor& x, const Tensor& w, const Opt& res, double
       y = out[0];
       if (res) r = out[1];
     } else {
-      norm_forward(x, w.contiguous(), res ? *res : Tensor(), eps, false, false, y, r, scale, rstd);
+      norm_forward(x, plain(w), res ? *res : Tensor(), eps, false, false, y, r, scale, rstd);
     }
   }
   return py::make_tuple(y, res ? r : x);
@@ -538,7 +545,7 @@ py::object add_rms_norm(const Tensor& x, const Tensor& w, const Opt& res, double
 py::object add_rms_norm_8bit(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
   if (!norm_ok(x, w, res, eps) || graph(Opt(x), Opt(w), res) || forward_mode(x, w, res)) return py::none();
   Tensor y, r, scale, rstd;
-  norm_forward(x, w.contiguous(), res ? *res : Tensor(), eps, true, false, y, r, scale, rstd);
+  norm_forward(x, plain(w), res ? *res : Tensor(), eps, true, false, y, r, scale, rstd);
   return py::make_tuple(y, scale, res ? r : x);
 }
 
