@@ -96,9 +96,16 @@ class SequenceSSM(nn.Module):
                 x = gen.linear(y, layer.out_proj.weight, None)
             return mixer_ops.add_rms_norm(x, self.norm_weight, res, self.norm_eps)[0]
 
-    def _state_check(self, state: list):
+    def _state_check(self, state: list, batch: int, moves: bool):
+        """in front of the first layer, so that a refused step has moved no layer's state; moves: the state is written to, so it has to lie as it is written"""
         if len(state) != len(self.layers):
             raise ValueError(f'the state of {len(self.layers)} layers expected, got {len(state)}')
+        want = ((batch, self.kernel_size - 1, self.inner_dim), (batch, self.inner_dim, self.state_dim))
+        for k, pair in enumerate(state):
+            if len(pair) != 2 or any(tuple(t.shape) != w or t.dtype != torch.float32 for t, w in zip(pair, want)):
+                raise ValueError(f'layer {k}: a state of fp32 tensors {want[0]} and {want[1]} expected, got {[(tuple(t.shape), t.dtype) for t in pair]}')
+            if moves and not all(t.is_contiguous() and t.device == self.norm_weight.device and not t.requires_grad for t in pair):
+                raise ValueError(f'layer {k}: a step writes its state in place: contiguous tensors on {self.norm_weight.device} that want no gradient expected')
 
     @torch.no_grad()
     def prompt(self, x_BSF: Tensor, lengths: Tensor | None = None, state: list | None = None):
@@ -108,7 +115,7 @@ class SequenceSSM(nn.Module):
             raise ValueError(f'[B, S, {self.feature_dim}] with one epoch at least expected, got {tuple(x_BSF.shape)}')
         B, S, _ = x_BSF.shape
         state = self.init_state(B) if state is None else state
-        self._state_check(state)
+        self._state_check(state, B, False)
         behind = [[None, None] for _ in self.layers]
         seq = lambda t: t.unflatten(0, (B, S))   # noqa: E731
 
@@ -129,7 +136,7 @@ class SequenceSSM(nn.Module):
         """The newest epoch's features [B, F] -> mixed features [B, F]; `state` (init_state, or what prompt returned) moves on in place."""
         if x_BF.dim() != 2 or x_BF.shape[1] != self.feature_dim:
             raise ValueError(f'[B, {self.feature_dim}] expected, got {tuple(x_BF.shape)}')
-        self._state_check(state)
+        self._state_check(state, x_BF.shape[0], True)
 
         def conv(k, u, st):
             p = self.layers[k]
