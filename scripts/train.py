@@ -25,6 +25,8 @@ def main(argv=None) -> int:
     ap.add_argument('--synthetic-epochs', type=int, default=960, help='30-s epochs per synthetic recording (960 = 8 h)')
     ap.add_argument('--max-length-hours', type=int, default=10); ap.add_argument('--num-workers', type=int, default=4); ap.add_argument('--seed', type=int, default=42)
     a = ap.parse_args(argv)
+    if a.model == 'ppgnet' and a.sequence_mixer != 'cnn':
+        ap.error('--sequence-mixer belongs to --model wav2sleep: SleepPPGNet has no sequence mixer')
     import torch.distributed as dist
     world, rank, local = int(os.environ.get('WORLD_SIZE', 1)), int(os.environ.get('RANK', 0)), int(os.environ.get('LOCAL_RANK', 0))
     torch.cuda.set_device(local)
