@@ -99,7 +99,7 @@ class GenericForward:
             if share is not None:
                 fn.share = share
             if acc_ok:
-                fn.acc_ok = True
+                fn.acc_ok = acc_ok
             self.tape.append((out, tuple(inputs), fn))
 
     def _add(self, a, b):
@@ -143,7 +143,14 @@ class GenericForward:
             g_owned = id(g) in owned
             owned.discard(id(g))
             k0 = id(inputs[0]) if len(inputs) == 1 else None
-            if getattr(fn, 'acc_ok', False) and k0 in grads and id(grads[k0]) in owned:
+            acc = getattr(fn, 'acc_ok', False)
+            if acc == 'read' and k0 in grads:   # a norm whose input already has one: it reads that (others may share it) and writes the sum to a tensor of its own
+                old = grads[k0]
+                grads[k0], = fn(g, acc=old)
+                owned.discard(id(old))
+                owned.add(id(grads[k0]))
+                continue
+            if acc and k0 in grads and id(grads[k0]) in owned:
                 fn(g, acc=grads[k0])   # a convolution whose input already has a gradient (the residual branch ran first): y += in the data-gradient launch
                 continue
             share = getattr(fn, 'share', None)   # 'all': the outputs ARE g (fan-out of an add); 'view': a view of g
@@ -779,12 +786,11 @@ class GenericForward:
             self._rec(r, (x, res), lambda g: (g, g), share='all')
 
         def bw(g, acc=None):   # acc: the gradient that r already has as the next residual, added in the same launch
-            gx = acc if acc is not None else torch.empty_like(r)
-            gw = torch.empty_like(w)
-            lib.add_norm_bwd(r, w, rstd, g.contiguous(), acc, gx, gw, eps)
+            gx, gw = torch.empty_like(r), torch.empty_like(w)
+            lib.add_norm_bwd(r, w, rstd, g.contiguous(), None if acc is None else acc.contiguous(), gx, gw, eps)
             self._pgrad(wp, gw)
             return (gx,)
-        self._rec(y, (r,), bw, acc_ok=True)
+        self._rec(y, (r,), bw, acc_ok='read')
         return y, r
 
     def _short_conv(self, x, wp, bp):
