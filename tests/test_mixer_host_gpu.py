@@ -1,6 +1,7 @@
 """The host side of the state space mixer's operators: what torch may hand them beside plain tensors."""
 import pytest
 import torch
+import torch.fx.experimental.proxy_tensor
 from torch.autograd import forward_ad
 
 import wav2sleep_amd as W
@@ -98,3 +99,29 @@ def test_a_conjugates_imaginary_part_of_one_channel():
     c = torch.complex(rnd(1, 2, 6, 1), rnd(2, 2, 6, 1))
     x, w = c.conj().imag, rnd(3, 1, 4)
     assert x.is_neg() and torch.equal(W.short_conv(x, w), W.short_conv(x.clone(), w))
+
+
+@pytest.mark.filterwarnings('ignore')
+@pytest.mark.parametrize('name', OPERATORS)
+def test_a_trace_is_refused(name):
+    """a trace records dispatched operators only: it would hold the allocation of the result and not the launch that fills it"""
+    f, kw = calls()[name]
+    first = next(iter(kw))
+    out = lambda o: o[0].float() if isinstance(o, tuple) else o   # noqa: E731
+    with pytest.raises(W.lib.W2SError, match='trace'):
+        torch.jit.trace(lambda t: out(f(**{**kw, first: t})), (kw[first],), check_trace=False)
+    with pytest.raises(W.lib.W2SError, match='trace'):
+        torch.fx.experimental.proxy_tensor.make_fx(lambda t: out(f(**{**kw, first: t})))(kw[first])
+    f(**kw)
+
+
+def test_a_compiled_caller_runs_them_as_they_are():
+    """no trace: a compiler leaves the call in the program, also with gradients, and other dispatch modes go on around it"""
+    from torch.utils.flop_counter import FlopCounterMode
+    f, kw = calls()['short_conv']
+    x = kw['x'].clone().requires_grad_(True)
+    run = lambda t: (f(**{**kw, 'x': 2 * t}) + 1).sum()   # noqa: E731
+    want = torch.autograd.grad(run(x), x)[0]
+    assert torch.equal(torch.autograd.grad(torch.compile(run, backend='aot_eager')(x), x)[0], want)
+    with FlopCounterMode(display=False):
+        assert torch.equal(torch.autograd.grad(run(x), x)[0], want)

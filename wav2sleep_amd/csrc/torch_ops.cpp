@@ -6,6 +6,8 @@
 
 #include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
@@ -70,6 +72,13 @@ bool sized(const Tensor& t) {   // every size within 2^30: the descriptors hold 
   for (const int64_t n : t.sizes())
     if (n > (1 << 30)) return false;
   return true;
+}
+// jit.trace, make_fx and export record dispatched operators: they would keep a result's allocation and not the launch that fills it
+bool traced() {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer)) return true;
+  return TorchDispatchModeTLS::any_modes_set() && (TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY) || TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::FAKE));
 }
 bool io(const Tensor& t, int64_t dim) { return t.defined() && t.is_cuda() && t.layout() == at::kStrided && code(t) >= 0 && t.dim() == dim && sized(t); }
 
@@ -203,7 +212,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
 };
 
 bool conv_ok(const Tensor& x, const Tensor& w, const Opt& bias, const Opt& state, int64_t dim) {
-  if (!io(x, dim) || !w.defined() || w.dim() != 2) return false;
+  if (!io(x, dim) || !w.defined() || w.dim() != 2 || traced()) return false;
   const int64_t D = x.size(-1), K = w.size(1);
   return D >= 1 && K >= 1 && K <= 8 && is(w, x, at::kFloat, {D, K}) && is(bias, x, at::kFloat, {D}) && is(state, x, x.scalar_type(), {x.size(0), K - 1, D});
 }
@@ -370,7 +379,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
 };
 
 bool ssm_ok(const Tensor& u, const Tensor& dt, const Tensor& A, Tensor& B, Tensor& C, const Opt& D, const Opt& z, const Opt& bias, const Opt& state, int64_t dim) {
-  if (!io(u, dim) || !A.defined() || A.dim() != 2 || !B.defined() || !C.defined()) return false;
+  if (!io(u, dim) || !A.defined() || A.dim() != 2 || !B.defined() || !C.defined() || traced()) return false;
   if (B.dim() == dim) B = B.unsqueeze(-2);
   if (C.dim() == dim) C = C.unsqueeze(-2);
   if (B.dim() != dim + 1) return false;
@@ -523,7 +532,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
 bool norm_ok(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
   if (!x.defined() || !x.is_cuda() || code(x) < 0 || x.layout() != at::kStrided || x.dim() < 1 || x.size(-1) < 1 || x.size(-1) > (1 << 30) || x.numel() / x.size(-1) > 0x7fffffff || !(eps >= 0.0))
     return false;
-  return is(w, x, at::kFloat, {x.size(-1)}) && (!res || is(*res, x, x.scalar_type(), x.sizes()) || is(*res, x, at::kFloat, x.sizes()));
+  return !traced() && is(w, x, at::kFloat, {x.size(-1)}) && (!res || is(*res, x, x.scalar_type(), x.sizes()) || is(*res, x, at::kFloat, x.sizes()));
 }
 
 py::object add_rms_norm(const Tensor& x, const Tensor& w, const Opt& res, double eps) {
@@ -560,6 +569,7 @@ PYBIND11_MODULE(_w2s_torch, m) {
     }
   });
   m.def("bind", &bind);
+  m.def("traced", &traced);
   m.def("short_conv", &short_conv);
   m.def("short_conv_step", &short_conv_step);
   m.def("ssm_scan", &ssm_scan);

@@ -93,6 +93,8 @@ def no_forward_mode(what, *ts):
 
 def _refused(what, *ts):
     no_forward_mode(what, *ts)
+    if _ops().traced():
+        raise lib.W2SError(f'{what} cannot be traced: a trace would hold its results without their values')
     raise lib.W2SError(f'{what}: arguments refused (dense tensors are wanted)')
 
 
