@@ -410,7 +410,8 @@ int w2s_causal_normalize_host(const double* x, long n, double sampling_freq, dou
  * No call of the reference stands behind these: they are a recurrent alternative to its SequenceCNN (models/wav2sleep.py:349-390), with a
  * form for one position at a time.  Activations are fp32, bf16 or fp16 (`dtype`), channels-last, channel stride 1, any other strides (given
  * in ELEMENTS); outputs are contiguous; parameters and states of the scan are fp32.  lengths: device int32 [B] or NULL; position t of
- * sequence b exists if t < lengths[b] (clamped to [0, L] on the device): outputs and gradients behind it are 0 and inputs there are not read. */
+ * sequence b exists if t < lengths[b] (clamped to [0, L] on the device): outputs and gradients behind it are 0, and what the inputs hold there
+ * (up to L, as far as the scan loads) does not matter. */
 #define W2S_F32 0
 #define W2S_BF16 1
 #define W2S_F16 2

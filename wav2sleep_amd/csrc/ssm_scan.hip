@@ -13,9 +13,10 @@
 // gate are computed once per quad (the lane of position t mod 4) and broadcast by DPP.  B and C of a tile are staged in LDS in fp32, once per workgroup.
 // A tile's global loads are issued one tile ahead.  Where even that leaves CUs idle (few sequences, few channels) the sequence is cut into
 // segments: a first launch walks them for their end states alone, the second folds the ones in front of its own segment first.
-// Bound: the vector units (counters: 72 % busy forward, 66 - 76 % backward; 13.4 M and 33.1 M wave instructions), not HBM.  Measured, N = 16, gated: 16 nights
+// Bound: the vector units (counters of 16 nights: 67 % busy both ways; 13.4 M and 33.1 M wave instructions), not HBM.  Measured, N = 16, gated: 16 nights
 // x 960 x 256 fp32 (65 MB) 38 us forward = 1.7 TB/s, with the backward 149 us (130 MB by the least count, 0.9 TB/s); 4 x 2047 x 1536 bf16 in three groups
-// 124 + 330 us; one row of 16384 x 512 bf16 107 us.  One state a lane and positions one after another, without tiles, took 58 us for a night.
+// 124 + 330 us; one row of 16384 x 512 bf16 107 us, of which the end states of its segments are about four tenths.  One state a lane and positions one after
+// another, without tiles, took 58 us for a night.
 #include "mix_io.h"
 
 namespace {
@@ -72,7 +73,9 @@ __device__ __forceinline__ float sum_quads_of_row(float v) {   // over the four 
 // WIDE where there is at most one workgroup a CU and nothing to gain from cutting sequences: the forward then takes sixteen waves, which hide each other's LDS
 // and barrier waits, and the backward eight with a long walk each (sixteen: 109 us against 100).  With more workgroups than CUs, eight waves of at most 128
 // registers a lane, so that a CU holds two workgroups and the last round of them is short.  fp32, L = 960, D = 256, N = 16, wide / not, forward and with the
-// backward: 256 workgroups 38 / 43 and 141 / 165 us, 288 workgroups 72 / 59 and 262 / 228 us, 512 workgroups 74 / 60 and 284 / 252 us.
+// backward: 256 workgroups 38 / 43 and 141 / 165 us, 288 workgroups 72 / 59 and 262 / 228 us, 512 workgroups 74 / 60 and 284 / 252 us.  One workgroup more than
+// there are CUs costs half as much again: some CU then has two, which share its vector units, and the others wait for it; up to 512 it costs no more.  (256 and 288
+// workgroups of 512 channels 39 and 59 us, with the backward 145 and 232; 240 and 300 of 3000 positions and 8 states in bf16 77 and 122, 295 and 494.)
 // From eight states a lane on the registers of a walk leave one shape; at 16 states a lane TT = 4 (forward of N = 64, 16 x 960 x 256: 174 us; TT = 8 spills: 276).
 template <int NPL, bool WIDE> struct FwdShape { static constexpr int W = NPL <= 4 && WIDE ? 16 : 8, TT = NPL <= 8 ? 8 : 4, SIMD = NPL <= 4 ? 4 : 2; };
 template <int NPL, bool WIDE> struct BwdShape { static constexpr int W = 8, TT = NPL == 16 || (NPL <= 4 && !WIDE) ? 4 : 8, SIMD = NPL <= 4 && !WIDE ? 4 : 2; };
@@ -801,7 +804,7 @@ bool launches(int64_t blocks, int threads) { return blocks * threads <= 0xffffff
 
 int npl_of(int N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
 // Segments a sequence is cut into.  Cutting costs a second walk for the end states (half of a whole one), so it pays only where the workgroups of whole
-// sequences leave half of the 256 CUs idle or more: then up to two workgroups a CU, of two tiles at least.  fp32, L = 960, D = 256, cut / whole, forward and
+// sequences leave half of the 256 CUs idle or more: then up to two workgroups a CU, of two tiles at least.  fp32, L = 960, D = 256, N = 16, cut / whole, forward and
 // with the backward: 16 workgroups 20 / 36 and 66 / 134 us, 128 workgroups 33 / 37 and 111 / 139 us, 192 workgroups 45 / 37 and 149 / 140 us; one row of
 // 16384 x 512 bf16 113 / 515 and 352 / 1967 us.
 int segments(int64_t blocks, int ntile) {

@@ -14,8 +14,14 @@ Sizes go up to 2^30 and a launch has fewer than 2^32 threads; a call beyond that
 16-bit result is rounded once.  Everything runs on the current stream of the tensors' device, allocates from torch's allocator, never synchronises, and
 records into a hipGraph.  CPU tensors raise (lib.W2SError): there is no CPU path.
 
-lengths (int32 [B], on the device): sequence b ends in front of position lengths[b], clamped to [0, L].  Inputs at and behind the end are not read,
-results and gradients there are 0, and a returned state is the one at the end (the initial state for a length of 0).
+lengths (int32 [B], on the device): sequence b ends in front of position lengths[b], clamped to [0, L].  What the inputs hold at and behind the end, NaN
+too, has no part in anything (the memory has to be there: a tile's loads run on to L); results and gradients there are 0, and a returned state is the one at
+the end (the initial state for a length of 0).
+
+A scan's backward takes scratch memory of 8 n bytes a position and block of 16 channels of a group, n being N rounded up to 8, 16, 32 or 64 (n / 2 bytes a
+position and channel where groups fill their blocks; 8 n for groups of a single channel), and its forward keeps n floats a channel every 32 or 64 positions.
+A backward that a hipGraph captures wants leaves that no living eager graph holds (detached ones will do).  jit.trace, make_fx and export raise; torch.compile
+calls the operators between its graphs.  No other argument of a step may overlap its `state_out`.
 """
 from __future__ import annotations
 
@@ -227,7 +233,8 @@ def ssm_step(u: Tensor, dt: Tensor, A: Tensor, B: Tensor, C: Tensor, state: Tens
 
 def add_rms_norm(x: Tensor, weight: Tensor, residual: Tensor | None = None, eps: float = 1e-5):
     """r = x + residual, y = r / sqrt(mean(r^2) + eps) * weight over the last dimension; returns (y, r).  residual: x's type or fp32 (a residual stream
-    in 32 bits), which is r's type; y has x's.  The sum is fp32 and y comes from it before r is rounded.  residual=None: r is x itself."""
+    in 32 bits), which is r's type; y has x's.  The sum is fp32 and y comes from it before r is rounded.  So is the mean of its squares: values beyond 1e19
+    (with eps = 0 also a row below 1e-19) leave its range.  residual=None: r is x itself."""
     out = _ops().add_rms_norm(x, weight, residual, eps)
     if out is None:
         _norm_check(x, weight, residual, eps)
