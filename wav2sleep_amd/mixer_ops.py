@@ -93,7 +93,7 @@ def _state_check(state, state_out):
 
 
 def no_forward_mode(what, *ts):
-    if torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise lib.W2SError(f'{what} has no forward-mode derivative: an argument carries a tangent')
 
 
