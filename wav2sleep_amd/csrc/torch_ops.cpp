@@ -8,7 +8,9 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "../../include/w2s.h"
@@ -111,6 +113,19 @@ void no_forward_mode(const variable_list& g) {   // of gradients that arrive at 
     if (forward_mode(t)) throw Failure("this operator's gradient has no forward-mode derivative: a gradient that arrived carries a tangent");
 }
 
+// A capture cannot take in the default stream, and torch hands a leaf's gradient over on the stream where the leaf first came into a graph that still lives: a
+// backward that is captured while an eager graph of the same leaves lives ends the process inside the engine.  It is refused here, in front of that.
+void no_captured_eager_leaf() {
+  const auto node = torch::autograd::get_current_node();
+  for (size_t i = 0; node && i < node->num_outputs(); ++i) {
+    const auto& to = node->next_edge(i).function;
+    if (!to || !node->task_should_compute_output(i) || !dynamic_cast<torch::autograd::AccumulateGrad*>(to.get())) continue;
+    const auto on = to->stream();
+    if (on && on->id() == 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      throw Failure("a backward cannot be captured while an eager graph of the same leaves lives: drop that graph, or use detached leaves");
+  }
+}
+
 // The gradients are kernels' results: a graph through them (create_graph) has to end in an error, not in a constant
 variable_list first_order(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -169,6 +184,7 @@ struct ShortConv : torch::autograd::Function<ShortConv> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_forward_mode(g);
+    no_captured_eager_leaf();
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &w = s[1], &bias = s[2], &state = s[3], &lengths = s[4];
     const int64_t k = ctx->saved_data["k"].toInt();
@@ -340,6 +356,7 @@ struct SsmScan : torch::autograd::Function<SsmScan> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_forward_mode(g);
+    no_captured_eager_leaf();
     const auto v = ctx->get_saved_variables();
     const Ssm s{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], v[9]};
     const int64_t k = ctx->saved_data["k"].toInt();
@@ -485,6 +502,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     no_forward_mode(g);
+    no_captured_eager_leaf();
     const auto s = ctx->get_saved_variables();
     const Tensor &x = s[0], &res = s[1], &w = s[2], &rstd = s[3], &first = x.defined() ? x : res;
     const int64_t k = ctx->saved_data["k"].toInt(), C = w.size(0);

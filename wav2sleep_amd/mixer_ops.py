@@ -20,8 +20,8 @@ the end (the initial state for a length of 0).
 
 A scan's backward takes scratch memory of 8 n bytes a position and block of 16 channels of a group, n being N rounded up to 8, 16, 32 or 64 (n / 2 bytes a
 position and channel where groups fill their blocks; 8 n for groups of a single channel), and its forward keeps n floats a channel every 32 or 64 positions.
-A backward that a hipGraph captures wants leaves that no living eager graph holds (detached ones will do).  jit.trace, make_fx and export raise; torch.compile
-calls the operators between its graphs.  No other argument of a step may overlap its `state_out`.
+A backward that a hipGraph captures wants leaves that no living eager graph of the default stream holds (detached ones will do), and raises otherwise.
+jit.trace, make_fx and export raise; torch.compile calls the operators between its graphs.  No other argument of a step may overlap its `state_out`.
 """
 from __future__ import annotations
 
