@@ -67,3 +67,11 @@ def test_autograd_through_the_model():
     for k, p in model.named_parameters():
         want = mod.trainer.views[p]
         assert float((got[k] - want).norm()) <= 1e-5 * float(want.norm()) + 1e-9, k   # (two forms of the loss' own gradient, the same launches behind them)
+
+
+@pytest.mark.filterwarnings('ignore')
+def test_a_trace_of_the_mixer_is_refused():
+    m, x = mixer(**SIZES[0]), torch.randn(2, 3, 16, device='cuda')
+    for f in (m, lambda t: m.prompt(t)[0]):
+        with pytest.raises(W.lib.W2SError, match='trace'):
+            torch.jit.trace(f, (x,), check_trace=False)

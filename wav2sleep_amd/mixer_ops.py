@@ -49,11 +49,17 @@ def _sizes(name, t):
         raise ValueError(f'{name}: sizes up to 2^30 expected, got {tuple(t.shape)}')
 
 
+def no_trace(what):
+    if _ops().traced():
+        raise lib.W2SError(f'{what}: no tracing here, a trace would hold results without their values')
+
+
 def _io(name, t):
     if not isinstance(t, Tensor):
         raise TypeError(f'{name}: a tensor is wanted, got {type(t).__name__}')
     if not t.is_cuda:
         raise lib.W2SError(f'{name}: wav2sleep_amd kernels need device tensors (no CPU path)')
+    no_trace(name)   # (in front of the checks of shapes, which a trace would record)
     if t.dtype not in lib.IO_DTYPES:
         raise ValueError(f'{name}: float32, bfloat16 or float16 expected, got {t.dtype}')
 
@@ -99,8 +105,6 @@ def no_forward_mode(what, *ts):
 
 def _refused(what, *ts):
     no_forward_mode(what, *ts)
-    if _ops().traced():
-        raise lib.W2SError(f'{what} cannot be traced: a trace would hold its results without their values')
     raise lib.W2SError(f'{what}: arguments refused (dense tensors are wanted)')
 
 

@@ -71,6 +71,7 @@ class SequenceSSM(nn.Module):
         from .wav2sleep import _gen
         gen = _gen(self)
         mixer_ops.no_forward_mode('SequenceSSM', x_BSF, *self.parameters())
+        mixer_ops.no_trace('SequenceSSM')
         with torch.cuda.device(self.norm_weight.device):
             return gen.sequence_ssm(self, x_BSF)
 
